@@ -20,7 +20,9 @@ CF_ERR_CUDA = -3
 CF_ERR_NO_DEVICE = -4
 CF_ERR_DEVICE_TIMEOUT = -5
 
-FMT_F32, FMT_F16, FMT_U8, FMT_BITS = 0, 1, 2, 3
+FMT_F32, FMT_F16, FMT_U8, FMT_BITS, FMT_BF16 = 0, 1, 2, 3, 4
+PAIR_HALF, PAIR_ADJACENT = 0, 1
+AXES_BLOCKS, AXES_CYCLIC = 0, 1
 RES_NONE, RES_ADD_POST, RES_AND_POST, RES_IAND_POST, RES_ADD_PRE, RES_Z_ONLY = 0, 1, 2, 3, 4, 5
 
 _P = ctypes.c_void_p
@@ -82,6 +84,16 @@ SIGNATURES = {
     "cf_pack_conv_weight_planes": (_INT, [_P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P]),
     "cf_token_mean_lif_fc": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _F,
                                     _F, _INT, _INT, _P]),
+    "cf_decay_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "cf_decay_attention": (_INT, [_P, _P, _P, _P, _INT, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64,
+                                  _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                  _I64, _I64, _F, _P, _I64, _P]),
+    "cf_decay_attention_step": (_INT, [_P, _P, _P, _P, _INT, _P, _P, _P, _P, _I64, _I64, _I64,
+                                       _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                       _I64, _I64, _F, _P]),
+    "cf_qk_norm_rope": (_INT, [_P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                               _I64, _I64, _I64, _I64, _I64, _P, _INT, _I64, _P, _I64,
+                               ctypes.POINTER(_I32), _INT, _INT, _INT, _P, _P, _INT, _F, _P]),
     "cf_set_wait_limit": (_INT, [ctypes.c_uint32]),
     "cf_test_arm_stalled_load": (_INT, [_INT]),
     "cf_avgpool_fc": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),

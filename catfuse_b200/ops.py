@@ -13,8 +13,9 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import (FMT_BITS, FMT_F16, FMT_F32, FMT_U8, RES_ADD_POST, RES_ADD_PRE,
-                   RES_AND_POST, RES_IAND_POST, RES_NONE, RES_Z_ONLY, CatfuseNativeError)
+from ._lib import (AXES_BLOCKS, AXES_CYCLIC, FMT_BF16, FMT_BITS, FMT_F16, FMT_F32, FMT_U8,
+                   PAIR_ADJACENT, PAIR_HALF, RES_ADD_POST, RES_ADD_PRE, RES_AND_POST,
+                   RES_IAND_POST, RES_NONE, RES_Z_ONLY, CatfuseNativeError)
 
 __all__ = [
     "LIFConfig", "ssa_lif", "lif_fwd", "bn_lif", "add_lif", "avgpool_lif", "pack_tbchw", "unpack_bhwtc",
@@ -22,7 +23,8 @@ __all__ = [
     "conv_geometry", "prescan", "prescan_conv_tiles", "conv_chunk", "avgpool_fc", "maxpool_bhwtc",
     "pad16", "SPIKE_FORMATS", "RES_MODES", "PRECISIONS", "pack_conv_weight_split",
     "pack_im2col_split", "im2col_weight_split", "split_prescale", "check_device_error",
-    "set_wait_limit", "token_mean_lif_fc", "conv_bn_lif_dual",
+    "set_wait_limit", "token_mean_lif_fc", "conv_bn_lif_dual", "qk_norm_rope", "decay_attention",
+    "decay_attention_step",
 ]
 
 # Operand precision of the fused conv: "fp16" = fp16 weights (spikes are exact
@@ -625,3 +627,222 @@ def conv_bn_lif_dual(x: torch.Tensor, wp: torch.Tensor, scale: torch.Tensor, shi
               _ptr(v_in), _ptr(v_out), out.data_ptr(), _ptr(v_in2), _ptr(v_out2), out2.data_ptr(),
               int(Cout1), T, B, H, W, Cin_p, Cout, KH, KW, stride, pad, *lif.args(), _stream())
     return out, out2
+
+
+# ---------------------------------------------------------------------------
+# decayed linear attention over token streams
+# ---------------------------------------------------------------------------
+
+_HALF_FORMATS = {torch.float16: FMT_F16, torch.bfloat16: FMT_BF16}
+_PAIRINGS = {"half": PAIR_HALF, "adjacent": PAIR_ADJACENT}
+_AXIS_ORDERS = {"blocks": AXES_BLOCKS, "cyclic": AXES_CYCLIC}
+
+
+def _on_device(t: torch.Tensor, name: str, dtype=None):
+    """A CUDA tensor of the current device (the launch goes to its stream)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise CatfuseNativeError(f"{name} must be a CUDA tensor (no CPU path exists)",
+                                 _lib.CF_ERR_INVALID_ARG)
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current device")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    return t
+
+
+def _head_strides(t: torch.Tensor, name: str):
+    """Token and head strides of t[..., H, D]: the leading axes must collapse
+    into one token axis and channels must be adjacent."""
+    st, shape = t.stride(), t.shape
+    if not t.numel():
+        return 0, 0
+    if shape[-1] != 1 and st[-1] != 1:
+        raise ValueError(f"the channels of {name} must be adjacent")
+    token = 0
+    span = 1
+    for i in range(len(shape) - 3, -1, -1):
+        if shape[i] == 1:
+            continue
+        if span == 1:
+            token = st[i]
+        elif st[i] != span * token:
+            raise ValueError(f"the leading axes of {name} must collapse into one token axis")
+        span *= shape[i]
+    return token, st[-2]
+
+
+def _states(t: torch.Tensor, name: str, shape):
+    _on_device(t, name, torch.float32)
+    if t.dim() != 4 or tuple(t.shape[1:]) != shape:
+        raise ValueError(f"{name} must be [rows, {shape[0]}, {shape[1]}, {shape[2]}] fp32")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.shape[0]
+
+
+def _decay_args(q, k, v, log_decay, out, lead):
+    """Shape checks that prompts and single tokens share -> (fmt, Hq, Hk, Dk, Dv, out)."""
+    _on_device(q, "q")
+    fmt = _HALF_FORMATS.get(q.dtype)
+    if fmt is None:
+        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
+    _on_device(k, "k", q.dtype)
+    _on_device(v, "v", q.dtype)
+    if q.dim() != lead + 2 or k.dim() != lead + 2 or v.dim() != lead + 2:
+        raise ValueError(f"q, k and v must have {lead + 2} dimensions")
+    if k.shape[:-2] != q.shape[:-2] or v.shape[:-1] != k.shape[:-1] or k.shape[-1] != q.shape[-1]:
+        raise ValueError("q [..., Hq, Dk], k [..., Hk, Dk] and v [..., Hk, Dv] do not match")
+    Hq, Dk = q.shape[-2:]
+    Hk, Dv = v.shape[-2:]
+    _on_device(log_decay, "log_decay", torch.float32)
+    if log_decay.numel() != Hk or not log_decay.is_contiguous():
+        raise ValueError(f"log_decay must hold Hk={Hk} contiguous values")
+    shape = (*q.shape[:-1], Dv)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    else:
+        _on_device(out, "out", q.dtype)
+        if tuple(out.shape) != shape:
+            raise ValueError(f"out must be {list(shape)}")
+    return fmt, Hq, Hk, Dk, Dv, out
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                    scale: Optional[float] = None, s_in: Optional[torch.Tensor] = None,
+                    s_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                    cu_seqlens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """Causal linear attention with a decay per head over whole prompts:
+    ``S_t = exp(log_decay) S_{t-1} + k_t^T v_t``, ``o_t = scale q_t S_t``.
+
+    q [B, L, Hq, Dk], k [B, L, Hk, Dk], v [B, L, Hk, Dv], fp16 or bf16, any strides
+    whose leading axes collapse; or, with ``cu_seqlens`` (int32 [S + 1] on the
+    device), packed sequences q [N, Hq, Dk], ....  Hq is a multiple of Hk and
+    log_decay [Hk] fp32 at most 0.  scale defaults to Dk ** -0.5.  s_in / s_out
+    [rows, Hk, Dk, Dv] fp32 carry the state (s_out may be s_in); ``slots`` int32
+    names the row of each sequence (outside the rows: start from zeros, store
+    nothing).  Returns out [..., Hq, Dv]."""
+    packed = cu_seqlens is not None
+    fmt, Hq, Hk, Dk, Dv, out = _decay_args(q, k, v, log_decay, out, 1 if packed else 2)
+    if packed:
+        _on_device(cu_seqlens, "cu_seqlens", torch.int32)
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or not cu_seqlens.is_contiguous():
+            raise ValueError("cu_seqlens must be a contiguous [S + 1] tensor")
+        S, L, N = cu_seqlens.numel() - 1, 0, q.shape[0]
+    else:
+        S, L = q.shape[:2]
+        N = S * L
+    rows = [_states(t, n, (Hk, Dk, Dv)) for t, n in ((s_in, "s_in"), (s_out, "s_out")) if t is not None]
+    if len(rows) == 2 and rows[0] != rows[1]:
+        raise ValueError("s_in and s_out must have the same number of rows")
+    if slots is not None:
+        _on_device(slots, "slots", torch.int32)
+        if tuple(slots.shape) != (S,) or not slots.is_contiguous():
+            raise ValueError(f"slots must be a contiguous [{S}] tensor")
+    need = _lib.load().cf_decay_attention_workspace(S, N, Hk, Dk, Dv)
+    if need < 0:
+        _lib.check(need, "cf_decay_attention_workspace")
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.call("cf_decay_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), fmt,
+              log_decay.data_ptr(), _ptr(s_in), _ptr(s_out), _ptr(slots), rows[0] if rows else 0,
+              _ptr(cu_seqlens), S, L, N, Hq, Hk, Dk, Dv, *_head_strides(q, "q"),
+              *_head_strides(k, "k"), *_head_strides(v, "v"), *_head_strides(out, "out"),
+              float(Dk ** -0.5 if scale is None else scale), _ptr(ws), need, _stream())
+    return out
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                         log_decay: torch.Tensor, s_in: torch.Tensor,
+                         s_out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                         slots: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """:func:`decay_attention` for one token of each of B sequences: q [B, Hq, Dk],
+    k [B, Hk, Dk], v [B, Hk, Dv] -> out [B, Hq, Dv].  The states s_in
+    [rows, Hk, Dk, Dv] are updated in place, or written to ``s_out``; ``slots``
+    int32 [B] names the row of each sequence (outside the rows: a padding entry,
+    zero output, no state touched)."""
+    fmt, Hq, Hk, Dk, Dv, out = _decay_args(q, k, v, log_decay, out, 1)
+    B = q.shape[0]
+    rows = _states(s_in, "s_in", (Hk, Dk, Dv))
+    if s_out is None:
+        s_out = s_in
+    elif _states(s_out, "s_out", (Hk, Dk, Dv)) != rows:
+        raise ValueError("s_in and s_out must have the same number of rows")
+    if slots is not None:
+        _on_device(slots, "slots", torch.int32)
+        if tuple(slots.shape) != (B,) or not slots.is_contiguous():
+            raise ValueError(f"slots must be a contiguous [{B}] tensor")
+    _lib.call("cf_decay_attention_step", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+              fmt, log_decay.data_ptr(), s_in.data_ptr(), s_out.data_ptr(), _ptr(slots), rows, B,
+              Hq, Hk, Dk, Dv, *_head_strides(q, "q"), *_head_strides(k, "k"),
+              *_head_strides(v, "v"), *_head_strides(out, "out"),
+              float(Dk ** -0.5 if scale is None else scale), _stream())
+    return out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                 inv_freq: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, norm: bool = True, eps: float = 1e-6,
+                 sections=None, axis_order: str = "blocks", pairing: str = "half",
+                 q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """Per-head RMS norm of q [..., Hq, D] and k [..., Hk, D] (fp16 or bf16) and
+    the rotation of their first 2 * len(inv_freq) channels, in one pass ->
+    (q_out, k_out); q_out may be q and k_out k.
+
+    positions: int32 or int64, one per token ([...]) or, for several axes (time,
+    height, width), [axes, ...]; sections[a] = number of rotated pairs that
+    follow axis a, in whole blocks (``axis_order="blocks"``) or one pair of each
+    axis in turn (``"cyclic"``).  Pair p is channels (p, p + rot/2)
+    (``pairing="half"``) or (2p, 2p + 1) (``"adjacent"``).  q_weight / k_weight
+    [D] fp32 scale the norm (None = 1); ``norm=False`` only rotates."""
+    _on_device(q, "q")
+    fmt = _HALF_FORMATS.get(q.dtype)
+    if fmt is None:
+        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
+    _on_device(k, "k", q.dtype)
+    if q.dim() < 2 or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise ValueError("q [..., Hq, D] and k [..., Hk, D] do not match")
+    lead, (Hq, D), Hk = q.shape[:-2], q.shape[-2:], k.shape[-2]
+    N = lead.numel()
+    _on_device(inv_freq, "inv_freq", torch.float32)
+    if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous vector")
+    pairs = inv_freq.numel()
+    sections = (pairs,) if sections is None else tuple(int(x) for x in sections)
+    axes = len(sections)
+    _on_device(positions, "positions")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+    if positions.shape != lead and positions.shape != (axes, *lead) or positions.numel() != axes * N:
+        raise ValueError(f"positions must be {[*lead]} or {[axes, *lead]}")
+    if not positions.is_contiguous():
+        raise ValueError("positions must be contiguous")
+    for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _need(w, n, torch.float32)
+            if w.numel() != D:
+                raise ValueError(f"{n} must have D={D} elements")
+    outs = []
+    for t, o, n in ((q, q_out, "q_out"), (k, k_out, "k_out")):
+        if o is None:
+            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        else:
+            _on_device(o, n, t.dtype)
+            if o.shape != t.shape:
+                raise ValueError(f"{n} must be {[*t.shape]}")
+        outs.append(o)
+    import ctypes
+    _lib.call("cf_qk_norm_rope", q.data_ptr(), k.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(),
+              fmt, N, Hq, Hk, D, *_head_strides(q, "q"), *_head_strides(k, "k"),
+              *_head_strides(outs[0], "q_out"), *_head_strides(outs[1], "k_out"),
+              positions.data_ptr(), 32 if positions.dtype == torch.int32 else 64, N,
+              inv_freq.data_ptr(), 2 * pairs, (ctypes.c_int32 * axes)(*sections), axes,
+              _lookup(_AXIS_ORDERS, axis_order, "axis_order"), _lookup(_PAIRINGS, pairing, "pairing"),
+              _ptr(q_weight), _ptr(k_weight), int(bool(norm)), float(eps), _stream())
+    return tuple(outs)
+
+
+def _lookup(table, key, name):
+    if key not in table:
+        raise ValueError(f"{name} must be one of {tuple(table)}")
+    return table[key]

@@ -51,6 +51,13 @@ extern "C" {
 #define CF_FMT_F16  1   /* float16                                       */
 #define CF_FMT_U8   2   /* uint8 (spikes / spike counts)                  */
 #define CF_FMT_BITS 3   /* bit-packed spikes: bit (i%32) of word i/32     */
+#define CF_FMT_BF16 4   /* bfloat16 (attention operators)                 */
+
+/* ---- rotated pairs of cf_qk_norm_rope ------------------------------------ */
+#define CF_PAIR_HALF     0  /* channels (p, p + rot/2)                      */
+#define CF_PAIR_ADJACENT 1  /* channels (2p, 2p + 1)                        */
+#define CF_AXES_BLOCKS   0  /* all pairs of axis 0, then all of axis 1, ... */
+#define CF_AXES_CYCLIC   1  /* one pair of each axis in turn                */
 
 /* ---- residual modes of the fused conv epilogue -------------------------- */
 #define CF_RES_NONE      0  /* out = s                                      */
@@ -373,6 +380,71 @@ CF_API int cf_conv_bn_lif_planes(const void* x, const void* wq, const float* sca
 CF_API int cf_pack_conv_weight_planes(const float* w, void* wq, int64_t Cout, int64_t Cin,
                                       int64_t KH, int64_t KW, int64_t Cin_p, float prescale,
                                       void* stream);
+
+/* ---- decayed linear attention over token streams -------------------------- */
+
+/* Spiking self-attention has no softmax (cf_ssa_lif), so its causal form is a
+ * recurrence: each head owns a state that leaks from token to token like a
+ * membrane.  With l = exp(log_decay[h]), per head h:
+ *     S_t = l * S_{t-1} + k_t^T v_t          S [Dk][Dv] fp32
+ *     o_t = scale * q_t S_t
+ * log_decay [Hk] fp32 is at most 0 for a leak (-inf: nothing is kept).  The Hq
+ * query heads come in Hk groups; query head h reads the state of head
+ * h / (Hq / Hk).  q, k, v and out are fp16 or bf16 (`fmt`), states fp32
+ * [rows][Hk][Dk][Dv].  Tensors are given by the element strides of a token
+ * (`_st`) and of a head (`_sh`), channels adjacent, so q, k and v may be slices
+ * of one fused projection.  No counterpart in the reference, whose attention
+ * (models/spikformer_github.py:147-153) sees all tokens of an image at once.
+ * Dk and Dv: multiples of 8, at most 128. */
+
+/* Whole prompts.  N tokens in S sequences: sequence s is tokens
+ * [s*L, (s+1)*L) (N = S*L) when cu_seqlens is NULL, else
+ * [cu_seqlens[s], cu_seqlens[s+1]) (S + 1 int32 on the device, ascending; values
+ * are clamped to [0, N], tokens outside every sequence are not written).
+ * A sequence starts from its row of s_in (NULL: zeros) and leaves its state
+ * in s_out (NULL: not stored), which may be s_in; a sequence without tokens
+ * copies its state.  slots (int32 [S], NULL: row = sequence) gives the row of each
+ * sequence among n_slots rows; a slot outside [0, n_slots) starts from zeros
+ * and stores nothing.  Rows of one call must differ.
+ * `workspace`: cf_decay_attention_workspace bytes, 16-byte aligned, free for
+ * reuse once the call's kernels have run.  A non-finite v reaches the outputs of
+ * its own sequence only. */
+CF_API int64_t cf_decay_attention_workspace(int64_t S, int64_t N, int64_t Hk, int64_t Dk, int64_t Dv);
+CF_API int cf_decay_attention(const void* q, const void* k, const void* v, void* out, int fmt,
+                              const float* log_decay, const float* s_in, float* s_out,
+                              const int32_t* slots, int64_t n_slots, const int32_t* cu_seqlens,
+                              int64_t S, int64_t L, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk,
+                              int64_t Dv, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                              int64_t v_st, int64_t v_sh, int64_t o_st, int64_t o_sh, float scale,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One token for each of B sequences: q [B][Hq][Dk], k [B][Hk][Dk], v and out
+ * likewise.  States as above, read from s_in and written to s_out (which may be
+ * s_in); a sequence whose slot lies outside [0, n_slots) is padding: its
+ * outputs are zero and no state is touched. */
+CF_API int cf_decay_attention_step(const void* q, const void* k, const void* v, void* out, int fmt,
+                                   const float* log_decay, const float* s_in, float* s_out,
+                                   const int32_t* slots, int64_t n_slots, int64_t B, int64_t Hq,
+                                   int64_t Hk, int64_t Dk, int64_t Dv, int64_t q_st, int64_t q_sh,
+                                   int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                                   int64_t o_st, int64_t o_sh, float scale, void* stream);
+
+/* Per-head RMS norm of queries and keys and their position rotation, in one
+ * pass.  q [N][Hq][D], k [N][Hk][D] and their outputs (which may be q and k) by
+ * strides, fp16 or bf16.  norm != 0: x / sqrt(mean(x^2) + eps) * weight, with
+ * q_weight / k_weight [D] fp32 (NULL = 1).  The first `rot` channels are rotated
+ * in pairs (CF_PAIR_*) by pos * inv_freq[p] (inv_freq [rot/2] fp32), where pos is
+ * the token's position on the pair's axis: positions holds `axes` (1 to 4)
+ * rows of N values of pos_bits (32 or 64) signed bits, pos_stride elements
+ * apart; sections[axes] (host memory) says how many pairs each axis has, and
+ * axis_order (CF_AXES_*) which they are.  D even and at most 256, rot even. */
+CF_API int cf_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int fmt,
+                           int64_t N, int64_t Hq, int64_t Hk, int64_t D, int64_t q_st, int64_t q_sh,
+                           int64_t k_st, int64_t k_sh, int64_t qo_st, int64_t qo_sh, int64_t ko_st,
+                           int64_t ko_sh, const void* positions, int pos_bits, int64_t pos_stride,
+                           const float* inv_freq, int64_t rot, const int32_t* sections, int axes,
+                           int axis_order, int pairing, const float* q_weight,
+                           const float* k_weight, int norm, float eps, void* stream);
 
 /* ---- bounded device-side waits ------------------------------------------- */
 

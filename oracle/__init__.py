@@ -22,10 +22,11 @@ from .prescan import prescan_rf, choose_group_size, select_tile_sizes
 from .ssa import ssa_lif
 from .nets import sew_resnet18_forward, spiking_resnet18_forward, make_resnet18_params
 from .spikformer import spikformer_forward
+from .decay import axis_of_pair, decay_attention, qk_norm_rope
 
 __all__ = [
     "lif_multistep", "lif_multistep_triton_form", "fold_bn", "conv_bn_lif",
     "conv_bn_lif_residual", "prescan_rf", "choose_group_size", "select_tile_sizes",
     "sew_resnet18_forward", "spiking_resnet18_forward", "make_resnet18_params", "ssa_lif",
-    "spikformer_forward",
+    "spikformer_forward", "decay_attention", "qk_norm_rope", "axis_of_pair",
 ]
