@@ -84,7 +84,7 @@ SIGNATURES = {
     "cf_pack_conv_weight_planes": (_INT, [_P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P]),
     "cf_token_mean_lif_fc": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _F,
                                     _F, _INT, _INT, _P]),
-    "cf_decay_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "cf_decay_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _INT]),
     "cf_decay_attention": (_INT, [_P, _P, _P, _P, _INT, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64,
                                   _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                   _I64, _I64, _F, _P, _I64, _P]),

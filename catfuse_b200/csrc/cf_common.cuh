@@ -20,6 +20,12 @@ int fail(int code, const char* fmt, ...);
 int check_cuda(cudaError_t e, const char* what);
 int check_launch(const char* what);
 int require_sm100();
+// Bounded-wait plumbing shared by the tensor-core kernels (cf_conv.cu): the
+// device error word of the current device (NULL if it has no address), the
+// limit of cf_set_wait_limit, and the one-shot of cf_test_arm_stalled_load.
+int32_t* device_error_word();
+uint32_t wait_limit();
+int take_stalled_load();
 
 // Site codes for g_dev_error.
 enum : int32_t {

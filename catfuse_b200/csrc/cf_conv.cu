@@ -414,6 +414,13 @@ int conv_bn_lif_impl(const void* x, const void* wp, const float* scale, const fl
   return CF_OK;
 }
 
+int32_t* device_error_word() { return dev_error_ptr(); }
+uint32_t wait_limit() {
+  const uint32_t lim = g_wait_limit.load(std::memory_order_relaxed);
+  return lim ? lim : kMaxPolls;
+}
+int take_stalled_load() { return g_stall_armed.exchange(0) ? 1 : 0; }
+
 }  // namespace cf
 
 using namespace cf;

@@ -1,44 +1,54 @@
-// cf_decay.cu — decayed linear attention over whole prompts:
+// cf_decay.cu — decayed linear attention over whole prompts (host side and the
+// small kernels; the tensor-core kernel is in cf_decay_kernels.cuh).
 //
 //   S_t = l S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t,   l = exp(log_decay[h])
 //
-// The plain recurrence: a CTA takes 32 columns of the state of one (sequence,
-// head) and walks its tokens, 16 at a time through shared memory.  A lane owns a
-// column, a warp an eighth of its rows, in registers.
-#include "cf_half.cuh"
+// A prompt is walked chunk by chunk by one CTA per (sequence, head).  Where that
+// leaves the GPU idle, sequences are cut into segments: one launch sums each
+// segment's own state from its k and v, a small one turns them into the states
+// that enter the segments, and the walk then runs per segment.
+#include "cf_decay_kernels.cuh"
+
+#include <atomic>
+#include <mutex>
 
 namespace cf {
-namespace {
+namespace decayk {
+// cf_decay_tc_{f16,bf16}.cu
+template <typename T>
+int launch_chunks(bool out, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                  const DecayArgs& a, int sms, cudaStream_t s);
+extern template int launch_chunks<__half>(bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+                                          const DecayArgs&, int, cudaStream_t);
+extern template int launch_chunks<__nv_bfloat16>(bool, const CUtensorMap&, const CUtensorMap&,
+                                                 const CUtensorMap&, const DecayArgs&, int, cudaStream_t);
+}  // namespace decayk
 
+namespace {
+using namespace decayk;
+
+constexpr int kMaxDim = 128;
+
+// --------------------------------------------------------------------------
+// Rows that a TMA load cannot start on (not 16-byte aligned): the recurrence
+// itself.  A CTA takes 32 columns of the state of one (sequence, head) and walks
+// its tokens, 16 at a time through shared memory.  A lane owns a column, a warp
+// an eighth of its rows, in registers.
+// --------------------------------------------------------------------------
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCols = 32;
 constexpr int kTok = 16;
-constexpr int kMaxDim = 128;
 constexpr int kRows = kMaxDim / kWarps;
 
-struct DecayArgs {
-  const void* q;
-  const void* k;
-  const void* v;
-  void* out;
-  const float* log_decay;
-  const float* s_in;
-  float* s_out;
-  const int32_t* slots;
-  const int32_t* cu;
-  int64_t n_slots, L, N, q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;
-  int Hq, Hk, Dk, Dv, n_slices;
-  float scale;
-};
-
 template <typename T>
-__global__ void __launch_bounds__(kThreads) decay_recurrent_kernel(const __grid_constant__ DecayArgs a) {
+__global__ void __launch_bounds__(kThreads) decay_recurrent_kernel(const __grid_constant__ DecayArgs a,
+                                                               int n_slices) {
   __shared__ float s_k[kTok][kMaxDim], s_q[kTok][kMaxDim], s_v[kTok][kCols];
   __shared__ float s_o[kWarps][kTok][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int slice = blockIdx.x % a.n_slices;
-  const int64_t sh = blockIdx.x / a.n_slices;
+  const int slice = blockIdx.x % n_slices;
+  const int64_t sh = blockIdx.x / n_slices;
   const int h = (int)(sh % a.Hk);
   const int64_t seq = sh / a.Hk;
   const int G = a.Hq / a.Hk;
@@ -111,15 +121,233 @@ __global__ void __launch_bounds__(kThreads) decay_recurrent_kernel(const __grid_
   }
 }
 
+// --------------------------------------------------------------------------
+// segments
+// --------------------------------------------------------------------------
+
+// The segments of packed sequences, in order: every sequence has one at least.
+// Entries that are left over have seq = -1.
+__global__ void __launch_bounds__(1024) decay_segments_kernel(const int32_t* cu, int S, int64_t N, int64_t seg_len,
+                                                              Seg* segs, int32_t* first, int n_segs) {
+  __shared__ int s_sum[32];
+  __shared__ int s_base;
+  griddep_wait();
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) s_base = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int s0 = 0; s0 < S; s0 += 1024) {
+    const int s = s0 + threadIdx.x;
+    int64_t t0 = 0, t1 = 0;
+    int n = 0;
+    if (s < S) {
+      t0 = min(max((int64_t)cu[s], (int64_t)0), N);
+      t1 = min(max((int64_t)cu[s + 1], t0), N);
+      n = t1 > t0 ? (int)((t1 - t0 + seg_len - 1) / seg_len) : 1;
+    }
+    int x = n;
+    for (int m = 1; m < 32; m <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, m);
+      if (lane >= m) x += y;
+    }
+    if (lane == 31) s_sum[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+      int y = s_sum[lane];
+      for (int m = 1; m < 32; m <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, y, m);
+        if (lane >= m) y += z;
+      }
+      s_sum[lane] = y;
+    }
+    __syncthreads();
+    int at = s_base + x - n + (warp ? s_sum[warp - 1] : 0);
+    if (s < S) {
+      first[s] = at;
+      for (int i = 0; i < n && at < n_segs; ++i, ++at) {
+        const int64_t b = t0 + i * seg_len;
+        segs[at] = Seg{(int32_t)b, (int32_t)min(b + seg_len, t1), s, i == n - 1};
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s_base += s_sum[31];
+    __syncthreads();
+  }
+  for (int i = s_base + threadIdx.x; i < n_segs; i += 1024) segs[i] = Seg{0, 0, -1, 0};
+  if (threadIdx.x == 0) first[S] = min(s_base, n_segs);
+}
+
+// A segment's own state L_r becomes the state that enters it:
+// E_0 = s_in (not stored), E_{r+1} = l^{seg_len} E_r + L_r.  One thread per four
+// entries of a (sequence, head); the states of a call fit the L2.
+__global__ void __launch_bounds__(256) decay_enter_kernel(const __grid_constant__ DecayArgs a,
+                                                          const int32_t* first) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int dd = a.Dk * a.Dv, parts = (dd + 1023) / 1024;
+  const int e = (int)(blockIdx.x % parts * 256 + threadIdx.x) * 4;
+  const int h = (int)(blockIdx.x / parts % a.Hk);
+  const int64_t seq = blockIdx.x / parts / a.Hk;
+  if (e >= dd) return;
+  const int64_t r0 = a.segs ? first[seq] : seq * a.n_seg;
+  const int n = a.segs ? first[seq + 1] - first[seq] : a.n_seg;
+  const int64_t slot = a.slots ? a.slots[seq] : seq;
+  float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (a.s_in && slot >= 0 && slot < a.n_slots)
+    run = *reinterpret_cast<const float4*>(a.s_in + (slot * a.Hk + h) * dd + e);
+  const float2 l = pow_hi_lo(a.log_decay[h], a.seg_len);
+  const int64_t step = (int64_t)a.Hk * dd;
+  float* p = a.seg_states + (r0 * a.Hk + h) * dd + e;
+  float4 own = n > 1 ? *reinterpret_cast<const float4*>(p) : run;
+  for (int r = 1; r < n; ++r) {
+    p += step;
+    float4 next = own;
+    if (r + 1 < n) next = *reinterpret_cast<const float4*>(p);
+    run.x = fmaf(l.x, run.x, fmaf(l.y, run.x, own.x));
+    run.y = fmaf(l.x, run.y, fmaf(l.y, run.y, own.y));
+    run.z = fmaf(l.x, run.z, fmaf(l.y, run.z, own.z));
+    run.w = fmaf(l.x, run.w, fmaf(l.y, run.w, own.w));
+    *reinterpret_cast<float4*>(p) = run;
+    own = next;
+  }
+}
+
+// --------------------------------------------------------------------------
+// host side
+// --------------------------------------------------------------------------
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 148;
+  }
+  return n;
+}
+
+struct Plan {
+  int64_t seg_len, n_segs, state_bytes, bytes;
+  int n_seg;  // segments of each sequence (dense)
+  bool split;
+};
+
+// How long the segments are.  Times in units of one chunk of a single query
+// head: the walk takes 1 for a chunk and its first query head and about 0.4 for
+// every further one, the pass that sums states 0.5, and the three launches of a
+// cut call cost about 8 more than the one of an uncut call.
+Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t Dv, bool packed, int sms) {
+  Plan p{};
+  const int64_t ctas = sms * ((Dk <= 64 && Dv <= 64) ? 2 : 1);
+  const int64_t units = S * Hk;
+  const double t_walk = 1.0 + 0.4 * ((double)Hq / Hk - 1.0), t_sum = 0.5, t_cut = 8.0;
+  p.n_segs = S;
+  p.n_seg = 1;
+  p.seg_len = N > kC ? (N + kC - 1) / kC * kC : kC;
+  if (S > 0 && N > 0) {
+    if (!packed) {
+      const int64_t ch = (N / S + kC - 1) / kC;
+      double best = 0;
+      for (int64_t n = 1; n <= ch && n <= 1024; ++n) {
+        const int64_t len = (ch + n - 1) / n;
+        if ((ch + len - 1) / len != n) continue;
+        const double waves = (double)((units * n + ctas - 1) / ctas);
+        const double waves_s = (double)((units * (n - 1) + sms - 1) / sms);
+        const double t = waves * len * t_walk + (n > 1 ? waves_s * len * t_sum + t_cut : 0.0);
+        if (n == 1 || t < best) {
+          best = t;
+          p.n_seg = (int)n;
+          p.seg_len = len * kC;
+        }
+      }
+      p.n_segs = S * p.n_seg;
+      p.split = p.n_seg > 1;
+    } else {
+      // Lengths are on the device: segments of an equal share of all chunks, so
+      // that one long sequence among short ones does not run alone at the end.
+      const int64_t share = (N / kC * Hk + ctas - 1) / ctas;
+      const int64_t len = share > 16 ? share : 16;
+      if (N > len * kC) {
+        p.seg_len = len * kC;
+        p.n_segs = S + N / p.seg_len;
+        p.split = true;
+      }
+    }
+  }
+  if (p.split) {
+    p.state_bytes = p.n_segs * Hk * Dk * Dv * 4;
+    p.bytes = p.state_bytes + (packed ? p.n_segs * (int64_t)sizeof(Seg) + (S + 1) * 4 : 0);
+    p.bytes = (p.bytes + 15) / 16 * 16;
+  }
+  return p;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// x[N][H][D] by strides, in boxes of 64 tokens x 64 channels of one head.  Heads
+// of a multiple of 64 channels bring their panels in one load.
+int make_map(CUtensorMap* m, int fmt, const void* x, int64_t N, int64_t H, int64_t D, int64_t st,
+             int64_t sh, int* panels) {
+  const bool whole = D % 64 == 0;
+  *panels = whole ? (int)(D / 64) : 1;
+  if (N == 1 && st % 8) st = 8;  // an axis of one entry: its stride is never taken
+  if (H == 1) sh = D;
+  cuuint64_t dims[4] = {(cuuint64_t)(whole ? 64 : D), (cuuint64_t)N, (cuuint64_t)*panels, (cuuint64_t)H};
+  cuuint64_t strides[3] = {(cuuint64_t)st * 2, 128, (cuuint64_t)sh * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)kC, (cuuint32_t)*panels, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  auto encode = encode_fn();
+  if (!encode) return fail(CF_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const CUresult r = encode(m, fmt == CF_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                            4, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(CF_ERR_CUDA, "tensor map (attention) failed: %d", (int)r);
+  return CF_OK;
+}
+
+// Whether TMA can read rows: 16-byte address and strides, strides within the
+// tensor map's range.
+bool tma_rows(const void* p, int64_t N, int64_t H, int64_t st, int64_t sh) {
+  const int64_t lim = (int64_t)1 << 38;
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (N == 1 || (st % 8 == 0 && st > 0 && st < lim)) &&
+         (H == 1 || (sh % 8 == 0 && sh > 0 && sh < lim));
+}
+
+template <typename Kern, typename... Args>
+int launch_after(Kern kernel, dim3 grid, int threads, cudaStream_t s, const char* what, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
 }  // namespace
 }  // namespace cf
 
 using namespace cf;
 
-extern "C" int64_t cf_decay_attention_workspace(int64_t S, int64_t N, int64_t Hk, int64_t Dk, int64_t Dv) {
-  if (S < 0 || N < 0 || Hk <= 0 || Dk <= 0 || Dv <= 0)
+extern "C" int64_t cf_decay_attention_workspace(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk,
+                                                int64_t Dv, int packed) {
+  if (S < 0 || N < 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || Dk <= 0 || Dv <= 0 || Dk > kMaxDim || Dv > kMaxDim)
     return fail(CF_ERR_INVALID_ARG, "bad attention shape");
-  return 0;
+  return make_plan(S, N, Hq, Hk, Dk, Dv, packed != 0, sm_count()).bytes;
 }
 
 extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, void* out, int fmt,
@@ -142,15 +370,64 @@ extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, v
     return fail(CF_ERR_INVALID_ARG, "q, k, v, out and log_decay must not be NULL");
   if (!slots && (s_in || s_out) && n_slots < S)
     return fail(CF_ERR_INVALID_ARG, "fewer states than sequences");
-  const int64_t slices = (Dv + kCols - 1) / kCols;
-  if (Hq > 65536 || S > 0x7FFFFFFF / (Hk * slices))
-    return fail(CF_ERR_UNSUPPORTED, "too many sequences or heads");
+  if (Hq > 65535 || N > 0x7FFFFFC0 || S > 0x7FFFFFFF / (Hk * 16))
+    return fail(CF_ERR_UNSUPPORTED, "too many tokens, sequences or heads");
+  for (const void* p : {(const void*)s_in, (const void*)s_out, (const void*)workspace})
+    if (reinterpret_cast<uintptr_t>(p) & 15)
+      return fail(CF_ERR_UNSUPPORTED, "states and workspace must be 16-byte aligned");
   if (int rc = require_sm100()) return rc;
-  DecayArgs a{q, k, v, out, log_decay, s_in, s_out, slots, cu_seqlens, n_slots, L, N, q_st, q_sh,
-              k_st, k_sh, v_st, v_sh, o_st, o_sh, (int)Hq, (int)Hk, (int)Dk, (int)Dv, (int)slices, scale};
-  const unsigned grid = (unsigned)(S * Hk * slices);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (fmt == CF_FMT_F16) decay_recurrent_kernel<__half><<<grid, kThreads, 0, st>>>(a);
-  else decay_recurrent_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a);
-  return check_launch("decay_attention launch");
+  DecayArgs a{};
+  a.q = q; a.k = k; a.v = v; a.out = out; a.log_decay = log_decay; a.s_in = s_in; a.s_out = s_out;
+  a.slots = slots; a.cu = cu_seqlens; a.n_slots = n_slots; a.L = L; a.N = N;
+  a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh;
+  a.o_st = o_st; a.o_sh = o_sh; a.Hq = (int)Hq; a.Hk = (int)Hk; a.Dk = (int)Dk; a.Dv = (int)Dv;
+  a.S = (int)S; a.scale = scale; a.n_seg = 1;
+
+  if (N == 0 || !tma_rows(q, N, Hq, q_st, q_sh) || !tma_rows(k, N, Hk, k_st, k_sh) ||
+      !tma_rows(v, N, Hk, v_st, v_sh)) {
+    const int slices = (int)((Dv + kCols - 1) / kCols);
+    const unsigned grid = (unsigned)(S * Hk * slices);
+    if (fmt == CF_FMT_F16) decay_recurrent_kernel<__half><<<grid, kThreads, 0, st>>>(a, slices);
+    else decay_recurrent_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, slices);
+    return check_launch("decay_attention launch");
+  }
+
+  const int sms = sm_count();
+  const Plan p = make_plan(S, N, Hq, Hk, Dk, Dv, cu_seqlens != nullptr, sms);
+  if (p.split && (!workspace || workspace_bytes < p.bytes))
+    return fail(CF_ERR_INVALID_ARG, "the workspace must have %lld bytes", (long long)p.bytes);
+  a.max_polls = wait_limit();
+  a.err = device_error_word();
+  if (!a.err) return fail(CF_ERR_CUDA, "device error word is not addressable");
+  a.drop_load = take_stalled_load();
+  a.n_seg = p.n_seg;
+  a.seg_len = p.seg_len;
+  a.seg_states = static_cast<float*>(workspace);
+  CUtensorMap mq, mk, mv;
+  if (int rc = make_map(&mq, fmt, q, N, Hq, Dk, q_st, q_sh, &a.qp)) return rc;
+  if (int rc = make_map(&mk, fmt, k, N, Hk, Dk, k_st, k_sh, &a.kp)) return rc;
+  if (int rc = make_map(&mv, fmt, v, N, Hk, Dv, v_st, v_sh, &a.vp)) return rc;
+  auto chunks = [&](bool with_out) {
+    return fmt == CF_FMT_F16 ? launch_chunks<__half>(with_out, mq, mk, mv, a, sms, st)
+                             : launch_chunks<__nv_bfloat16>(with_out, mq, mk, mv, a, sms, st);
+  };
+  if (p.split) {
+    int32_t* first = nullptr;
+    if (cu_seqlens) {
+      Seg* segs = reinterpret_cast<Seg*>(static_cast<char*>(workspace) + p.state_bytes);
+      first = reinterpret_cast<int32_t*>(segs + p.n_segs);
+      a.segs = segs;
+      if (int rc = launch_after(decay_segments_kernel, dim3(1), 1024, st, "decay segments launch", cu_seqlens,
+                                (int)S, N, p.seg_len, segs, first, (int)p.n_segs))
+        return rc;
+    }
+    a.n_units = (cu_seqlens ? p.n_segs : S * (p.n_seg - 1)) * Hk;
+    if (int rc = chunks(false)) return rc;
+    const dim3 grid((unsigned)((Dk * Dv + 1023) / 1024 * S * Hk));
+    if (int rc = launch_after(decay_enter_kernel, grid, 256, st, "decay states launch", a, (const int32_t*)first))
+      return rc;
+  }
+  a.n_units = p.n_segs * Hk;
+  return chunks(true);
 }

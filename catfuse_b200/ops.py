@@ -740,7 +740,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         _on_device(slots, "slots", torch.int32)
         if tuple(slots.shape) != (S,) or not slots.is_contiguous():
             raise ValueError(f"slots must be a contiguous [{S}] tensor")
-    need = _lib.load().cf_decay_attention_workspace(S, N, Hk, Dk, Dv)
+    need = _lib.load().cf_decay_attention_workspace(S, N, Hq, Hk, Dk, Dv, packed)
     if need < 0:
         _lib.check(need, "cf_decay_attention_workspace")
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None

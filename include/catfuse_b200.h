@@ -409,7 +409,8 @@ CF_API int cf_pack_conv_weight_planes(const float* w, void* wq, int64_t Cout, in
  * `workspace`: cf_decay_attention_workspace bytes, 16-byte aligned, free for
  * reuse once the call's kernels have run.  A non-finite v reaches the outputs of
  * its own sequence only. */
-CF_API int64_t cf_decay_attention_workspace(int64_t S, int64_t N, int64_t Hk, int64_t Dk, int64_t Dv);
+CF_API int64_t cf_decay_attention_workspace(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk,
+                                            int64_t Dv, int packed);
 CF_API int cf_decay_attention(const void* q, const void* k, const void* v, void* out, int fmt,
                               const float* log_decay, const float* s_in, float* s_out,
                               const int32_t* slots, int64_t n_slots, const int32_t* cu_seqlens,

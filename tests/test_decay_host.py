@@ -67,7 +67,8 @@ def test_entry_points_refuse_before_any_device():
                                       *st, 1.0, None, 0, None)
     assert prompt(q=None) == I and prompt(fmt=2) == I and prompt(hq=3) == I and prompt(N=5) == I
     assert prompt(rows=0) == I and prompt(dk=12) == _lib.CF_ERR_UNSUPPORTED and prompt(S=0, N=0) == _lib.CF_OK
-    assert lib.cf_decay_attention_workspace(-1, 1, 1, 64, 64) < 0
+    assert lib.cf_decay_attention_workspace(-1, 1, 1, 1, 64, 64, 0) < 0
+    assert lib.cf_decay_attention_workspace(1, 64, 1, 1, 64, 64, 0) == 0
 
     def rope(D=64, rot=64, sec=(32,), pos=32, order=0, pairing=0, q=16, fmt=1, N=1):
         return lib.cf_qk_norm_rope(q, 16, 16, 16, fmt, N, 2, 2, D, *st, 16, pos, N, 16, rot,
