@@ -239,7 +239,8 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
   Plan p{};
   const int64_t ctas = sms * ((Dk <= 64 && Dv <= 64) ? 2 : 1);
   const int64_t units = S * Hk;
-  const double t_walk = 1.0 + 0.4 * ((double)Hq / Hk - 1.0), t_sum = 0.5, t_cut = 8.0;
+  const double t_walk = 1.0 + 0.4 * ((double)Hq / Hk - 1.0), t_sum = 0.5, t_cut = 8.0,
+               t_unit = 3.0;
   p.n_segs = S;
   p.n_seg = 1;
   p.seg_len = N > kC ? (N + kC - 1) / kC * kC : kC;
@@ -252,7 +253,7 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
         if ((ch + len - 1) / len != n) continue;
         const double waves = (double)((units * n + ctas - 1) / ctas);
         const double waves_s = (double)((units * (n - 1) + sms - 1) / sms);
-        const double t = waves * len * t_walk + (n > 1 ? waves_s * len * t_sum + t_cut : 0.0);
+        const double t = waves * (len * t_walk + t_unit) + (n > 1 ? waves_s * (len * t_sum + t_unit) + t_cut : 0.0);
         if (n == 1 || t < best) {
           best = t;
           p.n_seg = (int)n;
@@ -404,6 +405,7 @@ extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, v
   a.n_seg = p.n_seg;
   a.seg_len = p.seg_len;
   a.seg_states = static_cast<float*>(workspace);
+  a.o_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && o_st % 8 == 0 && o_sh % 8 == 0;
   CUtensorMap mq, mk, mv;
   if (int rc = make_map(&mq, fmt, q, N, Hq, Dk, q_st, q_sh, &a.qp)) return rc;
   if (int rc = make_map(&mk, fmt, k, N, Hk, Dk, k_st, k_sh, &a.kp)) return rc;
@@ -422,12 +424,12 @@ extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, v
                                 (int)S, N, p.seg_len, segs, first, (int)p.n_segs))
         return rc;
     }
-    a.n_units = (cu_seqlens ? p.n_segs : S * (p.n_seg - 1)) * Hk;
+    a.n_units = (uint32_t)((cu_seqlens ? p.n_segs : S * (p.n_seg - 1)) * Hk);
     if (int rc = chunks(false)) return rc;
     const dim3 grid((unsigned)((Dk * Dv + 1023) / 1024 * S * Hk));
     if (int rc = launch_after(decay_enter_kernel, grid, 256, st, "decay states launch", a, (const int32_t*)first))
       return rc;
   }
-  a.n_units = p.n_segs * Hk;
+  a.n_units = (uint32_t)(p.n_segs * Hk);
   return chunks(true);
 }

@@ -16,21 +16,24 @@
 // Products per chunk (D = accumulator in TMEM, fp32):
 //   QK  [64 i][64 j]    A = Q (K-major),        B = K (K-major)
 //   KV  [dv][dk]        A = V' (MN-major),      B = K (MN-major)   V'_j = l^{n-1-j} v_j
-//   QS  [dv][64 i]      A = S^T (K-major),      B = Q (K-major)
+//   QS  [dv][64 i]      A = S^T,                B = Q (K-major)
 //   PV  [dv][64 i]      A = V (MN-major),       B = P (K-major)    P_ij = l^{i-j} QK_ij, j <= i
 // The outputs are built transposed (channels in lanes): with 64 tokens as M the
-// same products run at half rate.
+// same products run at half rate.  Channels are padded to 64 or 128 with the
+// zeros that TMA fills in.  With 128 of them V' and S^T go to the products from
+// TMEM, which halves what the products read from shared memory (the bound of
+// everything else that was tried: 128 bytes a cycle); with 64, an M = 64 product
+// takes them from shared memory and two CTAs share the SM.
 //
 // What is rounded to 16 bits on its way through a product, and how: V' carries
 // the state's precision, so it goes as three bf16 parts (24 bits) or two fp16
-// parts (22 bits); S and P only reach the 16-bit outputs and go as two parts, which
-// leaves the outputs' own rounding as their only error of that size (one part each
-// made it 1.4 times as large).  fp16 parts are scaled by powers of two (V' per chunk,
-// S per channel, P per row), so that neither a full state nor a small one leaves
-// fp16's range; bf16 has fp32's range.
+// parts (22 bits).  S and P reach only the 16-bit outputs and are rounded once,
+// which makes the outputs' error 1.42 times that of their own rounding alone.
+// In fp16 every row of V', S and P is scaled by a power of two of its own, so that
+// neither a full state nor a small one leaves the type's range; bf16 has fp32's.
 //
-// Warp roles: P warps (QK -> P), O warps (outputs), state warps (V', S), one TMA
-// warp, one MMA warp.
+// Warpgroups: P (QK -> P), O (outputs), S (state), V (V'; with 64 channels the S
+// warps do it), and one with the TMA and the MMA warp.
 #pragma once
 
 #include "cf_half.cuh"
@@ -43,7 +46,7 @@ namespace decayk {
 
 constexpr int kC = 64;            // tokens of a chunk
 constexpr int kTileBytes = kC * 128;  // 64 tokens x 64 channels of 16 bits, 128-byte swizzle
-constexpr int kSmallBytes = 3072;  // barriers and tables
+constexpr int kSmallBytes = 4096;  // barriers and tables
 
 enum : int32_t {
   ERR_SITE_DECAY_LOAD = 16,
@@ -51,7 +54,8 @@ enum : int32_t {
   ERR_SITE_DECAY_P = 18,
   ERR_SITE_DECAY_O = 19,
   ERR_SITE_DECAY_STATE = 20,
-  ERR_SITE_DECAY_ALIGN = 21,
+  ERR_SITE_DECAY_V = 21,
+  ERR_SITE_DECAY_ALIGN = 22,
 };
 
 struct Seg {  // one segment of one packed sequence
@@ -72,10 +76,11 @@ struct DecayArgs {
   float* seg_states;  // [segment][Hk][Dk][Dv]: a segment's own state, then the one that enters it
   int64_t n_slots, L, N, seg_len;  // seg_len: tokens of a segment, a multiple of 64 (or >= every length)
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;
-  int64_t n_units;    // segments x heads
+  uint32_t n_units;   // segments x heads, below 2^31
   int n_seg;          // segments of each sequence (dense)
   int Hq, Hk, Dk, Dv, S;
   int kp, vp, qp;     // panels of 64 channels that one load brings
+  int o_vec;          // rows of out start on 16 bytes
   float scale;
   uint32_t max_polls;
   int32_t* err;
@@ -88,18 +93,9 @@ struct Wait {
   volatile int* abort;
 };
 
-// One lane waits.
-__device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, int32_t site, const Wait& w) {
-  for (uint32_t i = 0; i < w.max_polls; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 255u && *w.abort) return false;
-  }
-  atomicCAS(w.err, 0, site);
-  *w.abort = 1;
-  return false;
-}
 // A whole warp waits (uniform result).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t site, const Wait& w) {
+#pragma unroll 1
   for (uint32_t i = 0; i < w.max_polls; ++i) {
     if (__any_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     if ((i & 255u) == 255u && __any_sync(0xffffffffu, *w.abort != 0)) return false;
@@ -110,6 +106,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_
   }
   __syncwarp();
   return false;
+}
+__device__ __forceinline__ bool warp_test(uint64_t* bar, uint32_t parity) {
+  return __any_sync(0xffffffffu, mbar_test_wait(bar, parity));
 }
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();
@@ -127,33 +126,152 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_
       : "memory");
 }
 
-// 16 columns of an accumulator.  M = 128: lane = row of the warp's quarter.
-// M = 64: the quarter's 16 rows sit in lanes 0-15; the upper half-warp takes
-// the columns 32 further on.
-template <int M>
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
+// Accumulator fragments.  One 16x256b load brings 16 lanes (rows) x 8 columns:
+// thread t of the warp holds row t / 4, columns 2 (t % 4) and + 1, then row
+// t / 4 + 8, the same columns; xN repeats that for the next columns.
+__device__ __forceinline__ void tmem_ld_frag8(uint32_t taddr, float (&r)[32]) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  if constexpr (M == 128) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
-          "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
-          "=r"(u[14]), "=r"(u[15])
-        : "r"(taddr)
-        : "memory");
-  } else {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x32bx2.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16], 32;\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
-          "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
-          "=r"(u[14]), "=r"(u[15])
-        : "r"(taddr)
-        : "memory");
-  }
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+        "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
+        "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]),
+        "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]),
+        "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(taddr)
+      : "memory");
+}
+// 32 columns, without waiting; tmem_wait16 hands the registers over.
+__device__ __forceinline__ void tmem_ld_frag4(uint32_t taddr, float (&r)[16]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+        "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
+        "=r"(u[14]), "=r"(u[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait16(float (&r)[16]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]),
+                 "+r"(u[7]), "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]),
+                 "+r"(u[14]), "+r"(u[15])::"memory");
+}
+// 16 rows x 32 words of a packed 16-bit operand: thread t holds row t / 4, word
+// t % 4 of every four, then row t / 4 + 8 (the fragment above, packed in pairs).
+__device__ __forceinline__ void tmem_st_frag8(uint32_t taddr, const uint32_t (&u)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
+      "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Four 8x8 blocks of 16-bit values; lane 8 m + r gives the address of row r of
+// block m.  A thread's registers are the fragment above; `_t`: transposed.
+__device__ __forceinline__ void stm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void stm4_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a),
+               "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void ldm4_t(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
+               : "memory");
+}
+
+// The MMA warp runs its loop with all lanes and one of them issues (`one`): in a
+// single lane's branch the compiler cannot keep descriptors in uniform registers,
+// and moving them there took 100 cycles a product.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+// D[tmem] (+)= A[smem] * B[smem]^T.
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]^T.
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(one)
+      : "memory");
+}
+
+// Two fp32 values at a time.
+struct alignas(8) F2 {
+  float x, y;
+};
+__device__ __forceinline__ uint64_t f2_bits(F2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ F2 f2_from(uint64_t r) {
+  F2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_from(r);
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return f2_from(r);
+}
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, F2{-1.f, -1.f}, a); }
+
+// Registers move between warpgroups: the sum stays within the launch's share.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Descriptor of an operand whose contiguous axis is M or N: panels of 64
@@ -183,13 +301,11 @@ struct Half2<__half> {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  static __device__ __forceinline__ float2 unpack(uint32_t u) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  static __device__ __forceinline__ F2 unpack(uint32_t u) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    return F2{f.x, f.y};
   }
-  // nonzero if one of the two is an infinity or NaN
-  static __device__ __forceinline__ uint32_t non_finite(uint32_t u) {
-    return ((u & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
-  }
+  static constexpr uint32_t kInf = 0x7C00;
 };
 template <>
 struct Half2<__nv_bfloat16> {
@@ -197,25 +313,19 @@ struct Half2<__nv_bfloat16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  static __device__ __forceinline__ float2 unpack(uint32_t u) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  static __device__ __forceinline__ F2 unpack(uint32_t u) {
+    return F2{__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)};
   }
-  static __device__ __forceinline__ uint32_t non_finite(uint32_t u) {
-    return ((u & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-  }
+  static constexpr uint32_t kInf = 0x7F80;
 };
 
-// x (two values) as `parts` 16-bit parts, largest first.
+// Two values as PARTS 16-bit parts each, largest first.
 template <typename T, int PARTS>
-__device__ __forceinline__ void split2(float a, float b, uint32_t (&out)[PARTS]) {
+__device__ __forceinline__ void split2(F2 a, uint32_t (&out)[PARTS]) {
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) {
-    out[p] = Half2<T>::pack(a, b);
-    if (p + 1 < PARTS) {
-      const float2 h = Half2<T>::unpack(out[p]);
-      a -= h.x;
-      b -= h.y;
-    }
+    out[p] = Half2<T>::pack(a.x, a.y);
+    if (p + 1 < PARTS) a = sub2(a, Half2<T>::unpack(out[p]));
   }
 }
 
@@ -227,6 +337,11 @@ __device__ __forceinline__ int fp16_shift(float m) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((127 + e) << 23); }
 
+__device__ __forceinline__ float exp2_fast(float x) {  // within 2^-22, and 1 at 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // l^n for n >= 0; 0^0 = 1 (log2 decays below -1e4 are one that keeps nothing).
 __device__ __forceinline__ float log2_decay(float log_decay) {
   const float l2 = log_decay * 1.4426950408889634f;
@@ -244,26 +359,38 @@ template <typename T, int DK, int DV, bool OUT>
 struct Cfg {
   static constexpr bool kFp16 = std::is_same<T, __half>::value;
   static constexpr int kVParts = kFp16 ? 2 : 3;
-  static constexpr int kCg = DK / 64;          // state warps per lane quarter
-  static constexpr int kStateWarps = 4 * kCg;
-  static constexpr int kOutWarps = OUT ? 8 : 0;  // P warps, then O warps
-  static constexpr int kWarps = kOutWarps + kStateWarps + 2;
-  static constexpr int kThreads = 32 * kWarps;
+  static constexpr bool kTm = DV == 128;       // V' and S^T in TMEM, V' by warps of its own
+  static constexpr int kHalves = DV / 64;      // 16-row halves of a warp's lanes
+  static constexpr int kCg = DK / 64;          // groups of 64 state columns
+  // warpgroups
+  static constexpr int kP = 0, kO = OUT ? 1 : -1, kS = OUT ? 2 : 0, kV = kTm ? kS + 1 : kS;
+  static constexpr int kCtl = kV + 1;
+  static constexpr int kThreads = 128 * (kCtl + 1);
+  static constexpr int kCtas = DV == 64 && DK == 64 ? (OUT ? 2 : 3) : 1;
   static constexpr int kKBytes = DK / 64 * kTileBytes;
   static constexpr int kVBytes = DV / 64 * kTileBytes;
   static constexpr int kSPart = DV * DK * 2;
-  static constexpr int kKvStages = OUT ? 2 : 3;
-  static constexpr int kQStages = OUT ? 2 : 0;
-  static constexpr int kVp = OUT ? 1 : 2;       // V' buffers
-  static constexpr int kScaleBytes = (OUT && kFp16) ? 4096 : 0;
-  static constexpr int kSmem = kKvStages * (kKBytes + kVBytes) + kQStages * kKBytes +
-                               kVp * kVParts * kVBytes + kScaleBytes +
-                               (OUT ? 2 * kSPart + 2 * kTileBytes : 0) + kSmallBytes;
-  static constexpr int kCtas = (OUT && DK == 64 && DV == 64) ? 2 : 1;
-  // TMEM columns: QK 64 | O from S 64 | O from P 64 | KV buffers
+  static constexpr int kVp = (!OUT && kTm) ? 2 : 1;  // V' and KV buffers
+  static constexpr int kKvStages = kCtas > 1 ? 2 : 4;
+  static constexpr int kQStages = OUT ? (kCtas > 1 ? 2 : 4) : 0;
+  static constexpr int kScaleBytes = kFp16 ? 4096 : 0;
+  static constexpr int kVpBytes = kTm ? 0 : kVp * kVParts * kVBytes;
+  static constexpr int kSBytes = (OUT && !kTm) ? kSPart : 0;
+  static constexpr int kStage = OUT ? kC * DV * 2 : 0;  // outputs on their way out
+  static constexpr int kSmem = kKvStages * (kKBytes + kVBytes) + kQStages * kKBytes + kVpBytes + kSBytes +
+                               (OUT ? kTileBytes : 0) + kStage + kScaleBytes + kSmallBytes;
+  // TMEM columns: QK 64 | O from S 64 | O from P 64 | KV | S | V'
   static constexpr int kColOs = 64, kColOp = 128, kColKv = OUT ? 192 : 0;
-  static constexpr int kColsUsed = kColKv + kVp * DK;
+  static constexpr int kColS = kColKv + kVp * DK;
+  static constexpr int kColV = kColS + ((OUT && kTm) ? DK / 2 : 0);
+  static constexpr int kColsUsed = kColV + (kTm ? kVp * kVParts * 32 : 0);
   static constexpr int kCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
+  // Registers of each warpgroup where the launch's even share does not do
+  // (threads x registers at launch, over 128: 5 x 96 and 4 x 64).
+  static constexpr bool kMove = OUT && (kTm || kCtas == 2);
+  static constexpr int kRegP = kTm ? 96 : 80, kRegO = kTm ? 96 : 64, kRegS = kTm ? 168 : 88, kRegV = 96,
+                       kRegCtl = 24;
+  static_assert(!kMove || kRegP + kRegO + kRegS + kRegCtl + (kTm ? kRegV : 0) <= (kTm ? 5 * 96 : 4 * 64), "registers");
 };
 
 struct Unit {
@@ -275,9 +402,9 @@ struct Unit {
 
 // Unit u of the grid (heads fastest).  Returns false if there is nothing in it.
 template <bool OUT>
-__device__ __forceinline__ bool get_unit(const DecayArgs& a, int64_t u, Unit& x) {
-  const int64_t sg = u / a.Hk;
-  x.h = (int)(u - sg * a.Hk);
+__device__ __forceinline__ bool get_unit(const DecayArgs& a, uint32_t u, Unit& x) {
+  const uint32_t sg = u / (uint32_t)a.Hk;
+  x.h = (int)(u - sg * (uint32_t)a.Hk);
   bool first, last;
   int64_t seg = sg;  // row of seg_states
   if (a.segs) {
@@ -294,9 +421,9 @@ __device__ __forceinline__ bool get_unit(const DecayArgs& a, int64_t u, Unit& x)
     x.len = (int)(min(max((int64_t)a.cu[sg + 1], x.t0), a.N) - x.t0);
     first = last = true;
   } else {
-    const int per = OUT ? a.n_seg : a.n_seg - 1;
+    const uint32_t per = OUT ? a.n_seg : a.n_seg - 1;
     x.seq = (int)(sg / per);
-    const int i = (int)(sg - (int64_t)x.seq * per);
+    const int i = (int)(sg - x.seq * per);
     seg = (int64_t)x.seq * a.n_seg + i;
     const int64_t off = (int64_t)i * a.seg_len;
     x.t0 = x.seq * a.L + off;
@@ -319,52 +446,99 @@ __device__ __forceinline__ bool get_unit(const DecayArgs& a, int64_t u, Unit& x)
   return true;
 }
 
+// The infinities and NaN among 16 channels of a tile of v: zeros in their place,
+// where PV would meet them as 0 * inf for earlier tokens; the O warps write NaN
+// from their token on.
+template <typename T>
+__device__ __forceinline__ void mark_non_finite(uint8_t* v, int d0, uint32_t chunk, uint32_t* bad,
+                                             volatile uint32_t* any) {
+#pragma unroll 1
+  for (int e = threadIdx.x & 31; e < kC * 16; e += 32) {
+    const int j = e >> 4, d = d0 + (e & 15);
+    uint16_t* at = reinterpret_cast<uint16_t*>(v + (d >> 6) * kTileBytes + j * 128 +
+                                               ((((d & 63) >> 3) ^ (j & 7)) << 4) + (d & 7) * 2);
+    if ((*at & 0x7FFFu) >= Half2<T>::kInf) {
+      *at = 0;
+      atomicMax(&bad[d], ((chunk + 1) << 6) + (63 - j));
+      *any = chunk + 1;
+    }
+  }
+  fence_async_shared();
+}
+
+// A warp's part of a chunk's outputs on its way out: kRow bytes of each token,
+// 16-byte vectors spread over all banks.
+template <int kRow>
+__device__ __forceinline__ int out_at(int row, int v) {
+  return row * kRow + ((v ^ ((row / (128 / kRow)) & (kRow / 16 - 1))) << 4);
+}
+template <int kRow>
+__device__ __forceinline__ void spoil_outputs(uint8_t* stage, const uint32_t* bad, uint32_t chunk) {
+  __syncwarp();
+#pragma unroll 1
+  for (int e = threadIdx.x & 31; e < kC * kRow / 2; e += 32) {
+    const int row = e / (kRow / 2), d = e % (kRow / 2);
+    const uint32_t b = bad[d];
+    if ((b >> 6) == chunk + 1 && row >= 63 - (int)(b & 63))
+      *reinterpret_cast<uint16_t*>(stage + out_at<kRow>(row, d >> 3) + (d & 7) * 2) = 0x7FFF;
+  }
+}
+template <typename T, int kRow>
+__device__ __forceinline__ void store_unaligned(const uint8_t* stage, T* to, int64_t st, int rows, int channels) {
+#pragma unroll 1
+  for (int e = threadIdx.x & 31; e < rows * (kRow / 2); e += 32) {
+    const int row = e / (kRow / 2), d = e % (kRow / 2);
+    if (d < channels)
+      to[(int64_t)row * st + d] = *reinterpret_cast<const T*>(stage + out_at<kRow>(row, d >> 3) + (d & 7) * 2);
+  }
+}
+
 template <typename T, int DK, int DV, bool OUT>
 __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, OUT>::kCtas)
     decay_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ DecayArgs a) {
   using K = Cfg<T, DK, DV, OUT>;
-  constexpr bool FP16 = K::kFp16;
-  constexpr int VP = K::kVp;
+  constexpr bool FP16 = K::kFp16, TM = K::kTm;
+  constexpr int VP = K::kVp, NH = K::kHalves;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sK = smem;
   uint8_t* sV = sK + K::kKvStages * K::kKBytes;
   uint8_t* sQ = sV + K::kKvStages * K::kVBytes;
   uint8_t* sVp = sQ + K::kQStages * K::kKBytes;
-  float* s_sscale = reinterpret_cast<float*>(sVp + VP * K::kVParts * K::kVBytes);  // fp16 only:
-  float* s_pscale = s_sscale + 256;  // [2][128] S's scales by chunk parity, [2][64] P's by item parity,
-  float* s_smax = s_pscale + 128;    // [2][2][128] maxima of half a channel of S
-  uint8_t* sS = sVp + VP * K::kVParts * K::kVBytes + K::kScaleBytes;
-  uint8_t* sP = sS + (OUT ? 2 * K::kSPart : 0);
-  uint8_t* small = sP + (OUT ? 2 * kTileBytes : 0);
+  uint8_t* sS = sVp + K::kVpBytes;
+  uint8_t* sP = sS + K::kSBytes;
+  uint8_t* sOut = sP + (OUT ? kTileBytes : 0);
+  float* s_sscale = reinterpret_cast<float*>(sOut + K::kStage);  // fp16 only: [2][128] S's scales by chunk,
+  float* s_pscale = s_sscale + 256;                              // [2][64] P's by item,
+  float* s_vscale = s_pscale + 128;                              // [4][128] V's by chunk
+  uint8_t* small = sOut + K::kStage + K::kScaleBytes;
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(small);
   uint64_t* kv_empty = kv_full + 4;
   uint64_t* q_full = kv_empty + 4;
   uint64_t* q_empty = q_full + 4;
   uint64_t* vp_full = q_empty + 4;
   uint64_t* ds_full = vp_full + 2;
-  uint64_t* qk_full = ds_full + 2;
+  uint64_t* ds_empty = ds_full + 2;
+  uint64_t* qk_full = ds_empty + 2;
   uint64_t* p_full = qk_full + 1;
-  uint64_t* o_full = p_full + 1;
+  uint64_t* p_empty = p_full + 1;
+  uint64_t* o_full = p_empty + 1;
   uint64_t* o_empty = o_full + 1;
   uint64_t* s_full = o_empty + 1;
   uint64_t* s_empty = s_full + 1;
-  uint64_t* p_sync = s_empty + 1;
-  uint64_t* st_sync = p_sync + 1;
-  uint64_t* done_bar = st_sync + 1;
+  uint64_t* done_bar = s_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile uint32_t* s_badany = reinterpret_cast<volatile uint32_t*>(tmem_slot + 2);  // [3]
-  float* s_vmax = reinterpret_cast<float*>(tmem_slot + 6);                    // [2][8] state warps
-  float* s_pow = reinterpret_cast<float*>(small + 512);                       // [2][128]: l^{n - 63}
-  // [3][DV]: chunk + 1 and, as 63 - j, the first token whose v is not finite in a
-  // channel.  Three, since v of chunk c + 2 may be looked at while chunk c is put out.
-  uint32_t* s_bad = reinterpret_cast<uint32_t*>(small + 1536);
+  volatile uint32_t* s_badany = reinterpret_cast<volatile uint32_t*>(tmem_slot + 2);  // [4]
+  // [4][DV]: chunk + 1 and, as 63 - j, the first token whose v is not finite in a
+  // channel.  More than one, since v is looked at ahead of the outputs.
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(small + 512);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int wg = warp >> 2, wq = warp & 3;  // warpgroup; the warp's TMEM lanes are 32 wq ..
   const Wait w{a.max_polls, a.err, abort_flag};
   const int G = a.Hq / a.Hk;
-  (void)s_sscale, (void)s_pscale, (void)s_smax;
+  (void)s_sscale, (void)s_pscale, (void)s_vscale;
 
   if (smem_u32(smem) & 1023u) {  // the swizzle is by address: without this alignment nothing may run
     if (threadIdx.x == 0) atomicCAS(a.err, 0, ERR_SITE_DECAY_ALIGN);
@@ -376,26 +550,26 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       mbar_init(&kv_empty[i], 1);
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
+      s_badany[i] = 0;
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&vp_full[i], K::kStateWarps);
+      mbar_init(&vp_full[i], 4);
       mbar_init(&ds_full[i], 1);
+      mbar_init(&ds_empty[i], 4);
     }
-    for (int i = 0; i < 3; ++i) s_badany[i] = 0;
     mbar_init(qk_full, 1);
     mbar_init(p_full, 4);
+    mbar_init(p_empty, 1);
     mbar_init(o_full, 1);
     mbar_init(o_empty, 4);
-    mbar_init(s_full, K::kStateWarps);
+    mbar_init(s_full, 4);
     mbar_init(s_empty, 1);
-    mbar_init(p_sync, 4);
-    mbar_init(st_sync, K::kStateWarps);
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  for (int i = threadIdx.x; i < 3 * DV; i += K::kThreads) s_bad[i] = 0;
-  constexpr int kTmaWarp = K::kWarps - 2, kMmaWarp = K::kWarps - 1;
+  for (int i = threadIdx.x; i < 4 * DV; i += K::kThreads) s_bad[i] = 0;
+  constexpr int kTmaWarp = K::kCtl * 4, kMmaWarp = kTmaWarp + 1;
   if (warp == kTmaWarp && lane == 0) {
     if (OUT) prefetch_tmap(&tmQ);
     prefetch_tmap(&tmK);
@@ -411,62 +585,70 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
   griddep_wait();
   griddep_launch_dependents();
   const uint32_t tmem = *tmem_slot;
+  const uint32_t tlane = tmem + ((uint32_t)(wq * 32) << 16);
+  const int fr = lane >> 2, fc = (lane & 3) * 2;  // a fragment's row and first column
 
-  if (warp == kTmaWarp) {
-    // ------------------------------------------------------------ loads
-    uint32_t cc = 0, it = 0;
-    uint32_t kv_used = 0, q_used = 0;  // parity of each stage's last load, + 2 once there was one
-    auto mark = [](uint32_t& used, int s, uint32_t parity) {
-      used = (used & ~(3u << (2 * s))) | ((2u | parity) << (2 * s));
-    };
-    bool ok = true, drop = a.drop_load && blockIdx.x == 0;
-    for (int64_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
-      Unit x;
-      if (!get_unit<OUT>(a, u, x)) continue;
-      for (int c = 0; c < x.len && ok; c += kC, ++cc) {
-        const int st = cc % K::kKvStages;
-        if (!(ok = warp_wait(&kv_empty[st], ((cc / K::kKvStages) & 1) ^ 1, ERR_SITE_DECAY_LOAD, w))) break;
-        const int t = (int)(x.t0 + c);
-        if (lane == 0 && !drop) {
-          mbar_arrive_expect_tx(&kv_full[st], K::kKBytes + K::kVBytes);
-          for (int p = 0; p < DK / 64; p += a.kp)
-            tma_load_4d(sK + st * K::kKBytes + p * kTileBytes, &tmK, &kv_full[st], a.kp == 1 ? 64 * p : 0, t, 0, x.h);
-          for (int p = 0; p < DV / 64; p += a.vp)
-            tma_load_4d(sV + st * K::kVBytes + p * kTileBytes, &tmV, &kv_full[st], a.vp == 1 ? 64 * p : 0, t, 0, x.h);
-        }
-        if (!drop) mark(kv_used, st, (cc / K::kKvStages) & 1);
-        drop = false;
-        __syncwarp();
-        if constexpr (OUT) {
-          for (int g = 0; g < G; ++g, ++it) {
-            const int qs = it % K::kQStages;
-            if (!(ok = warp_wait(&q_empty[qs], ((it / K::kQStages) & 1) ^ 1, ERR_SITE_DECAY_LOAD, w))) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&q_full[qs], K::kKBytes);
-              for (int p = 0; p < DK / 64; p += a.qp)
-                tma_load_4d(sQ + qs * K::kKBytes + p * kTileBytes, &tmQ, &q_full[qs], a.qp == 1 ? 64 * p : 0, t, 0,
-                            x.h * G + g);
+  if (wg == K::kCtl) {
+    if constexpr (K::kMove) regs_down<K::kRegCtl>();
+    if (warp == kTmaWarp) {
+      // ---------------------------------------------------------- loads
+      uint32_t cc = 0, it = 0;
+      uint32_t kv_used = 0, q_used = 0;  // parity of each stage's last load, + 2 once there was one
+      auto mark = [](uint32_t& used, int s, uint32_t parity) {
+        used = (used & ~(3u << (2 * s))) | ((2u | parity) << (2 * s));
+      };
+      bool ok = true, drop = a.drop_load && blockIdx.x == 0;
+      for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
+        Unit x;
+        if (!get_unit<OUT>(a, u, x)) continue;
+        for (int c = 0; c < x.len && ok; c += kC, ++cc) {
+          const int st = cc % K::kKvStages;
+          if (!(ok = warp_wait(&kv_empty[st], ((cc / K::kKvStages) & 1) ^ 1, ERR_SITE_DECAY_LOAD, w))) break;
+          const int t = (int)(x.t0 + c);
+          if (lane == 0 && !drop) {
+            mbar_arrive_expect_tx(&kv_full[st], K::kKBytes + K::kVBytes);
+            for (int p = 0; p < DK / 64; p += a.kp)
+              tma_load_4d(sK + st * K::kKBytes + p * kTileBytes, &tmK, &kv_full[st], a.kp == 1 ? 64 * p : 0, t, 0,
+                          x.h);
+            for (int p = 0; p < DV / 64; p += a.vp)
+              tma_load_4d(sV + st * K::kVBytes + p * kTileBytes, &tmV, &kv_full[st], a.vp == 1 ? 64 * p : 0, t, 0,
+                          x.h);
+          }
+          if (!drop) mark(kv_used, st, (cc / K::kKvStages) & 1);
+          drop = false;
+          __syncwarp();
+          if constexpr (OUT) {
+            for (int g = 0; g < G; ++g, ++it) {
+              const int qs = it % K::kQStages;
+              if (!(ok = warp_wait(&q_empty[qs], ((it / K::kQStages) & 1) ^ 1, ERR_SITE_DECAY_LOAD, w))) break;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&q_full[qs], K::kKBytes);
+                for (int p = 0; p < DK / 64; p += a.qp)
+                  tma_load_4d(sQ + qs * K::kKBytes + p * kTileBytes, &tmQ, &q_full[qs], a.qp == 1 ? 64 * p : 0, t, 0,
+                              x.h * G + g);
+              }
+              mark(q_used, qs, (it / K::kQStages) & 1);
+              __syncwarp();
             }
-            mark(q_used, qs, (it / K::kQStages) & 1);
-            __syncwarp();
           }
         }
       }
-    }
-    if (!ok) {
-      // the loads in flight land before the CTA ends
-      for (int s = 0; s < 4; ++s) {
-        for (uint32_t i = 0; (kv_used >> (2 * s) & 2u) && i < (1u << 16); ++i)
-          if (mbar_try_wait(&kv_full[s], kv_used >> (2 * s) & 1u)) break;
-        for (uint32_t i = 0; (q_used >> (2 * s) & 2u) && i < (1u << 16); ++i)
-          if (mbar_try_wait(&q_full[s], q_used >> (2 * s) & 1u)) break;
+      if (!ok) {
+        // the loads in flight land before the CTA ends
+        for (int s = 0; s < 4; ++s) {
+          for (uint32_t i = 0; (kv_used >> (2 * s) & 2u) && i < (1u << 16); ++i)
+            if (mbar_try_wait(&kv_full[s], kv_used >> (2 * s) & 1u)) break;
+          for (uint32_t i = 0; (q_used >> (2 * s) & 2u) && i < (1u << 16); ++i)
+            if (mbar_try_wait(&q_full[s], q_used >> (2 * s) & 1u)) break;
+        }
       }
-    }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------- MMA issuer
+      // Per chunk: KV, then for each query head PV, the next head's QK as soon
+      // as its operands are there, and QS.  P and V' of a chunk are ready early
+      // (QK of it ran in the chunk before), S last.
       constexpr uint32_t kIdQk = idesc<T>(64, 64, 0, 0);
-      constexpr uint32_t kIdKv = idesc<T>(DV, DK, 1, 1);
+      constexpr uint32_t kIdKv = idesc<T>(DV, DK, TM ? 0 : 1, 1);
       constexpr uint32_t kIdQs = idesc<T>(DV, 64, 0, 0);
       constexpr uint32_t kIdPv = idesc<T>(DV, 64, 1, 0);
       const uint64_t dQ = make_smem_desc(smem_u32(sQ), 128);
@@ -476,426 +658,549 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       const uint64_t dVpm = make_smem_desc_mn(smem_u32(sVp), kTileBytes);
       const uint64_t dS = make_smem_desc(smem_u32(sS), 128);
       const uint64_t dP = make_smem_desc(smem_u32(sP), 128);
-      const uint32_t dQk = tmem, dOs = tmem + K::kColOs, dOp = tmem + K::kColOp, dKv = tmem + K::kColKv;
+      const uint32_t one = elect_one();
+      const uint32_t tm = uniform(tmem);
       uint32_t cc = 0, it = 0, ns = 0;
       bool ok = true, qk_early = false;
       auto issue_qk = [&](uint32_t qs, uint32_t st) {
-        uint64_t ad = dQ + (uint64_t)(qs * (K::kKBytes >> 4)), bd = dKk + (uint64_t)(st * (K::kKBytes >> 4));
+        const uint64_t ad = dQ + (uint64_t)(qs * (K::kKBytes >> 4)), bd = dKk + (uint64_t)(st * (K::kKBytes >> 4));
 #pragma unroll
         for (int p = 0; p < DK / 64; ++p)
 #pragma unroll
           for (int s = 0; s < 4; ++s)
-            umma_f16(dQk, ad + p * (kTileBytes >> 4) + s * 2, bd + p * (kTileBytes >> 4) + s * 2, kIdQk, p + s > 0);
-        umma_commit(qk_full);
+            mma_ss(one, tm, ad + p * (kTileBytes >> 4) + s * 2, bd + p * (kTileBytes >> 4) + s * 2, kIdQk, p + s > 0);
+        mma_commit(one, qk_full);
       };
-      for (int64_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
+      for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
         if (!get_unit<OUT>(a, u, x)) continue;
-        for (int c = 0; c < x.len && ok; c += kC, ++cc) {
+        const int len = uniform(x.len), started = uniform(x.start != nullptr);
+        for (int c = 0; c < len && ok; c += kC, ++cc) {
           const uint32_t st = cc % K::kKvStages;
           const uint32_t vb = cc % VP;
-          if (!(ok = lane_wait(&kv_full[st], (cc / K::kKvStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
-          auto issue_kv = [&]() {
+          if (!(ok = warp_wait(&kv_full[st], (cc / K::kKvStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
+          if constexpr (OUT) {
+            if (!qk_early) {
+              const uint32_t qs = it % K::kQStages;
+              if (!(ok = warp_wait(&q_full[qs], (it / K::kQStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
+              tc_fence_after();
+              issue_qk(qs, st);
+            }
+            qk_early = false;
+          }
+          if (!(ok = warp_wait(&vp_full[vb], (cc / VP) & 1, ERR_SITE_DECAY_MMA, w))) break;
+          if (!(ok = warp_wait(&ds_empty[vb], ((cc / VP) & 1) ^ 1, ERR_SITE_DECAY_MMA, w))) break;
+          tc_fence_after();
+          {
             const uint64_t ad = dVpm + (uint64_t)(vb * K::kVParts * (K::kVBytes >> 4));
+            const uint32_t at = tm + K::kColV + vb * K::kVParts * 32;
             const uint64_t bd = dKm + (uint64_t)(st * (K::kKBytes >> 4));
+            const uint32_t d = tm + K::kColKv + vb * DK;
 #pragma unroll
             for (int p = K::kVParts - 1; p >= 0; --p)  // the small parts first
 #pragma unroll
-              for (int s = 0; s < 4; ++s)
-                umma_f16(dKv + vb * DK, ad + p * (K::kVBytes >> 4) + s * 128, bd + s * 128, kIdKv,
-                         p < K::kVParts - 1 || s > 0);
-            umma_commit(&ds_full[vb]);
-          };
+              for (int s = 0; s < 4; ++s) {
+                const uint32_t acc = p < K::kVParts - 1 || s > 0;
+                if constexpr (TM) mma_ts(one, d, at + p * 32 + s * 8, bd + s * 128, kIdKv, acc);
+                else mma_ss(one, d, ad + p * (K::kVBytes >> 4) + s * 128, bd + s * 128, kIdKv, acc);
+              }
+            mma_commit(one, &ds_full[vb]);
+          }
           if constexpr (!OUT) {
-            if (!(ok = lane_wait(&vp_full[vb], (cc / VP) & 1, ERR_SITE_DECAY_MMA, w))) break;
-            tc_fence_after();
-            issue_kv();
-            umma_commit(&kv_empty[st]);
+            mma_commit(one, &kv_empty[st]);
           } else {
-            const bool has_s = c > 0 || x.start != nullptr;
+            const bool has_s = c > 0 || started;
             for (int g = 0; g < G; ++g, ++it) {
               const uint32_t qs = it % K::kQStages;
-              if (!qk_early) {
-                if (!(ok = lane_wait(&q_full[qs], (it / K::kQStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
-                tc_fence_after();
-                issue_qk(qs, st);
+              if (!(ok = warp_wait(p_full, it & 1, ERR_SITE_DECAY_MMA, w))) break;
+              if (!(ok = warp_wait(o_empty, (it & 1) ^ 1, ERR_SITE_DECAY_MMA, w))) break;
+              tc_fence_after();
+              {
+                const uint64_t ad = dVm + (uint64_t)(st * (K::kVBytes >> 4));
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                  mma_ss(one, tm + K::kColOp, ad + s * 128, dP + s * 2, kIdPv, s > 0);
+                mma_commit(one, p_empty);
               }
-              qk_early = false;
-              if (g == 0) {
-                if (!(ok = lane_wait(&vp_full[vb], (cc / VP) & 1, ERR_SITE_DECAY_MMA, w))) break;
-                tc_fence_after();
-                issue_kv();
+              // QK's accumulator is free: P of this head is written
+              const bool same = g + 1 < G;
+              const uint32_t nq = (it + 1) % K::kQStages;
+              const uint32_t nst = same ? st : (cc + 1) % K::kKvStages;
+              if (same && !(ok = warp_wait(&q_full[nq], ((it + 1) / K::kQStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
+              if (same || (c + kC < len && warp_test(&q_full[nq], ((it + 1) / K::kQStages) & 1) &&
+                           warp_test(&kv_full[nst], ((cc + 1) / K::kKvStages) & 1))) {
+                issue_qk(nq, nst);
+                qk_early = !same;
               }
-              if (!(ok = lane_wait(o_empty, (it & 1) ^ 1, ERR_SITE_DECAY_MMA, w))) break;
+              if (!same) mma_commit(one, &kv_empty[st]);
               if (has_s) {
-                if (g == 0 && !(ok = lane_wait(s_full, ns & 1, ERR_SITE_DECAY_MMA, w))) break;
+                if (g == 0 && !(ok = warp_wait(s_full, ns & 1, ERR_SITE_DECAY_MMA, w))) break;
                 tc_fence_after();
                 const uint64_t bd = dQ + (uint64_t)(qs * (K::kKBytes >> 4));
 #pragma unroll
-                for (int part = 1; part >= 0; --part)
+                for (int p = 0; p < DK / 64; ++p)
 #pragma unroll
-                  for (int p = 0; p < DK / 64; ++p)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                      umma_f16(dOs, dS + part * (K::kSPart >> 4) + p * (DV * 128 >> 4) + s * 2,
-                               bd + p * (kTileBytes >> 4) + s * 2, kIdQs, part < 1 || p + s > 0);
-                if (g == G - 1) {
-                  umma_commit(s_empty);
+                  for (int s = 0; s < 4; ++s) {
+                    const uint64_t b = bd + p * (kTileBytes >> 4) + s * 2;
+                    if constexpr (TM) mma_ts(one, tm + K::kColOs, tm + K::kColS + p * 32 + s * 8, b, kIdQs, p + s > 0);
+                    else mma_ss(one, tm + K::kColOs, dS + p * (DV * 128 >> 4) + s * 2, b, kIdQs, p + s > 0);
+                  }
+                if (!same) {
+                  mma_commit(one, s_empty);
                   ++ns;
                 }
               }
-              if (!(ok = lane_wait(p_full, it & 1, ERR_SITE_DECAY_MMA, w))) break;
-              tc_fence_after();
-              // the next product with the queries, if its operands are there: it
-              // runs while the P warps of this one are done and PV is under way
-              {
-                const uint32_t nq = (it + 1) % K::kQStages;
-                const bool same = g + 1 < G;
-                const uint32_t nst = same ? st : (cc + 1) % K::kKvStages;
-                if ((same || c + kC < x.len) &&
-                    mbar_test_wait(&q_full[nq], ((it + 1) / K::kQStages) & 1) &&
-                    (same || mbar_test_wait(&kv_full[nst], ((cc + 1) / K::kKvStages) & 1))) {
-                  issue_qk(nq, nst);
-                  qk_early = true;
-                }
-              }
-              const uint64_t ad = dVm + (uint64_t)(st * (K::kVBytes >> 4));
-#pragma unroll
-              for (int part = 1; part >= 0; --part)
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                  umma_f16(dOp, ad + s * 128, dP + part * (kTileBytes >> 4) + s * 2, kIdPv, part < 1 || s > 0);
-              umma_commit(o_full);
-              umma_commit(&q_empty[qs]);
-              if (g == G - 1) umma_commit(&kv_empty[st]);
+              mma_commit(one, o_full);
+              mma_commit(one, &q_empty[qs]);
             }
           }
         }
       }
-      umma_commit(done_bar);
+      mma_commit(one, done_bar);
       for (uint32_t p = 0; p < kMaxPolls; ++p)
         if (mbar_try_wait(done_bar, 0)) break;
     }
-  } else if (OUT && warp < 4) {
+  } else if (OUT && wg == K::kP) {
     // ------------------------------------------------------------ QK -> P
-    // Lane: row i = 16 warp + lane % 16, columns 32 (lane / 16) + 0..31.
+    // Rows i = 16 wq + fr and + 8, columns j = 8 n + fc and + 1.
+    if constexpr (K::kMove) {
+      if constexpr (K::kRegP > (TM ? 96 : 64)) regs_up<K::kRegP>();
+    }
     if constexpr (OUT) {
-      uint32_t it = 0, nu = 0;
+      uint32_t it = 0;
       bool ok = true;
-      const int i = warp * 16 + (lane & 15), j0 = (lane >> 4) * 32;
-      for (int64_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
+      const int i = wq * 16 + fr;
+      // where the lane's row of an 8x8 block goes: block m = lane / 8 holds rows
+      // 8 (m % 2).., columns 8 (m / 2)..
+      const int si = wq * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+      const uint32_t prow = smem_u32(sP) + si * 128;
+      for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
         if (!get_unit<OUT>(a, u, x) || x.len == 0) continue;
-        float* pw = s_pow + (nu & 1) * 128;
-        for (int c = 0; c < x.len && ok; c += kC) {
-          for (int g = 0; g < G; ++g, ++it) {
-            if (!(ok = warp_wait(qk_full, it & 1, ERR_SITE_DECAY_P, w))) break;
-            tc_fence_after();
-            float r[32];
-            {
-              float(&lo)[16] = *reinterpret_cast<float(*)[16]>(&r[0]);
-              float(&hi)[16] = *reinterpret_cast<float(*)[16]>(&r[16]);
-              tmem_ld16<64>(tmem + ((uint32_t)(warp * 32) << 16), lo);
-              tmem_ld16<64>(tmem + ((uint32_t)(warp * 32) << 16) + 16, hi);
-            }
-            tc_fence_before();
-            // PV of the item before has read P, and the O warps the table two units back
-            if (it > 0 && !(ok = warp_wait(o_full, (it - 1) & 1, ERR_SITE_DECAY_P, w))) break;
-            if (c == 0 && g == 0) {
-              const float l2 = log2_decay(a.log_decay[x.h]);
-              const int n = threadIdx.x - 63;
-              pw[threadIdx.x] = n < 0 ? 0.f : exp2f(l2 * (float)n);
-              warp_arrive(p_sync);
-              if (!(ok = warp_wait(p_sync, nu & 1, ERR_SITE_DECAY_P, w))) break;
-            }
-            const float* f = pw + 63 + i - j0;
+        const float l2 = log2_decay(a.log_decay[x.h]);
+        F2 f[8][2];  // l^{i-j}, 0 above the diagonal
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float y = f[-j];
-              r[j] = y != 0.f ? r[j] * y : 0.f;  // never 0 * inf: what is masked is not looked at
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int d = i + 8 * r - 8 * n - fc;
+            f[n][r] = F2{d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1))};
+          }
+        const int items = (x.len + kC - 1) / kC * G;
+        for (int k = 0; k < items; ++k, ++it) {
+          if (!(ok = warp_wait(qk_full, it & 1, ERR_SITE_DECAY_P, w))) break;
+          tc_fence_after();
+          float q[32];
+          tmem_ld_frag8(tlane, q);
+          tc_fence_before();
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const F2 y = mul2(F2{q[4 * n + 2 * r], q[4 * n + 2 * r + 1]}, f[n][r]);
+              q[4 * n + 2 * r] = y.x;
+              q[4 * n + 2 * r + 1] = y.y;
+              // above the diagonal 0 * inf must not appear
+              if (i - fc < 8 * n - 8 * r) q[4 * n + 2 * r] = 0.f;
+              if (i - fc < 8 * n - 8 * r + 1) q[4 * n + 2 * r + 1] = 0.f;
             }
-            if constexpr (FP16) {
+          float undo[2] = {1.f, 1.f};
+          if constexpr (FP16) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
               float m = 0.f;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) m = fmaxf(m, fabsf(r[j]));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              for (int n = 0; n < 8; ++n) m = fmaxf(m, fmaxf(fabsf(q[4 * n + 2 * r]), fabsf(q[4 * n + 2 * r + 1])));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
               const int e = fp16_shift(m);
               const float up = pow2i(e);
+              undo[r] = pow2i(-e);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] *= up;
-              if (lane < 16) s_pscale[(it & 1) * 64 + i] = pow2i(-e);
+              for (int n = 0; n < 8; ++n) {
+                q[4 * n + 2 * r] *= up;
+                q[4 * n + 2 * r + 1] *= up;
+              }
             }
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-              uint32_t p[4][2];
-#pragma unroll
-              for (int z = 0; z < 4; ++z) split2<T, 2>(r[ch * 8 + 2 * z], r[ch * 8 + 2 * z + 1], p[z]);
-              const int off = i * 128 + (((j0 >> 3) + ch) ^ (i & 7)) * 16;
-              *reinterpret_cast<uint4*>(sP + off) = make_uint4(p[0][0], p[1][0], p[2][0], p[3][0]);
-              *reinterpret_cast<uint4*>(sP + kTileBytes + off) = make_uint4(p[0][1], p[1][1], p[2][1], p[3][1]);
-            }
-            fence_async_shared();
-            warp_arrive(p_full);
           }
+          // PV of the item before has read P
+          if (!(ok = warp_wait(p_empty, (it & 1) ^ 1, ERR_SITE_DECAY_P, w))) break;
+          if (FP16 && (lane & 3) == 0) {
+            s_pscale[(it & 1) * 64 + i] = undo[0];
+            s_pscale[(it & 1) * 64 + i + 8] = undo[1];
+          }
+#pragma unroll
+          for (int n = 0; n < 8; n += 2) {
+            uint32_t p[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) p[z] = Half2<T>::pack(q[4 * n + 2 * z], q[4 * n + 2 * z + 1]);
+            stm4(prow + (((n + (lane >> 4)) ^ (si & 7)) << 4), p[0], p[1], p[2], p[3]);
+          }
+          fence_async_shared();
+          warp_arrive(p_full);
         }
-        ++nu;
       }
     }
-  } else if (OUT && warp < 8) {
+  } else if (OUT && wg == K::kO) {
     // ------------------------------------------------------------ outputs
-    // DV = 128: lane = channel, all 64 tokens.  DV = 64: lane % 16 = channel,
-    // tokens 32 (lane / 16) + 0..31.
+    // Channels dv = (DV / 4) wq + 16 hh + fr and + 8, tokens 8 n + fc and + 1; put
+    // out through shared memory as rows of a token.
     if constexpr (OUT) {
-      uint32_t it = 0, cc = 0, nu = 0;
+      uint32_t it = 0, cc = 0;
       bool ok = true;
-      const int qd = warp & 3;
-      const int dv = DV == 128 ? qd * 32 + lane : qd * 16 + (lane & 15);
-      const int i0 = DV == 128 ? 0 : (lane >> 4) * 32;
-      const uint32_t ta = tmem + ((uint32_t)(qd * 32) << 16);
+      constexpr int kRow = DV / 4 * 2;       // bytes of a token's row of this warp: 64 or 32
+      constexpr int kVec = kRow / 16;        // 16-byte vectors of it
+      uint8_t* stage = sOut + wq * kC * kRow;
+      const uint32_t stage_u = smem_u32(stage);
       T* const out = static_cast<T*>(a.out);
-      for (int64_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
+      for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
         if (!get_unit<OUT>(a, u, x) || x.len == 0) continue;
-        const float* pw = s_pow + (nu & 1) * 128 + 64;  // l^{i+1}
+        const float l2 = log2_decay(a.log_decay[x.h]);
+        F2 grow[8];  // scale l^{i+1}
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+          grow[n] = F2{a.scale * exp2_fast(l2 * (float)(8 * n + fc + 1)), a.scale * exp2_fast(l2 * (float)(8 * n + fc + 2))};
         for (int c = 0; c < x.len && ok; c += kC, ++cc) {
           const bool has_s = c > 0 || x.start != nullptr;
-          const int n = min(kC, x.len - c);
+          const int n_tok = min(kC, x.len - c);
           for (int g = 0; g < G; ++g, ++it) {
             if (!(ok = warp_wait(o_full, it & 1, ERR_SITE_DECAY_O, w))) break;
             tc_fence_after();
-            T* const row = out + (x.t0 + c) * a.o_st + (int64_t)(x.h * G + g) * a.o_sh + dv;
-            float ss = a.scale;
-            if constexpr (FP16) ss *= s_sscale[(cc & 1) * 128 + dv];
-            int bad = kC;  // first token of the chunk whose v is not finite in this channel
-            if (s_badany[cc % 3] == cc + 1) {
-              const uint32_t b = s_bad[(cc % 3) * DV + dv];
-              if ((b >> 6) == cc + 1) bad = 63 - (int)(b & 63);
-            }
-            constexpr int NB = DV == 128 ? 4 : 2;
+            // groups of 16 channels x 32 tokens, one load ahead
+            auto group = [&](int q) { return tlane + ((uint32_t)(q / 2 * 16) << 16) + q % 2 * 32; };
+            float p[2][16], z[2][16];
+            tmem_ld_frag4(group(0) + K::kColOp, p[0]);
+            tmem_ld_frag4(group(0) + K::kColOs, z[0]);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              float r[16], s[16];
-              tmem_ld16<DV>(ta + K::kColOp + b * 16, r);
-              if (has_s) tmem_ld16<DV>(ta + K::kColOs + b * 16, s);
-              const int t = i0 + b * 16;
-              float o[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                float pr = a.scale;
-                if constexpr (FP16) pr *= s_pscale[(it & 1) * 64 + t + j];
-                o[j] = pr * r[j];
-                if (has_s) o[j] = fmaf(ss * pw[t + j], s[j], o[j]);
+            for (int q = 0; q < 2 * NH; ++q) {
+              const int hh = q / 2, cg = q % 2, b = q & 1;
+              tmem_wait16(p[b]);
+              tmem_wait16(z[b]);
+              if (q + 1 < 2 * NH) {
+                tmem_ld_frag4(group(q + 1) + K::kColOp, p[b ^ 1]);
+                tmem_ld_frag4(group(q + 1) + K::kColOs, z[b ^ 1]);
               }
-              if (b == NB - 1) {
+              float ss[2] = {1.f, 1.f};
+              if constexpr (FP16) {
+                ss[0] = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr];
+                ss[1] = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr + 8];
+              }
+              uint32_t o[4][2];
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                F2 pf = F2{a.scale, a.scale};
+                if constexpr (FP16) {
+                  const F2 ps = *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + cg * 32 + 8 * n + fc]);
+                  pf = mul2(pf, ps);
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  F2 y = mul2(F2{p[b][4 * n + 2 * r], p[b][4 * n + 2 * r + 1]}, pf);
+                  F2 x2 = F2{z[b][4 * n + 2 * r], z[b][4 * n + 2 * r + 1]};
+                  if constexpr (FP16) x2 = mul2(x2, F2{ss[r], ss[r]});
+                  if (has_s) y = fma2(grow[cg * 4 + n], x2, y);
+                  o[n][r] = Half2<T>::pack(y.x, y.y);
+                }
+              }
+              if (q == 2 * NH - 1) {  // accumulators and scales are read
                 tc_fence_before();
                 warp_arrive(o_empty);
               }
-              if (bad < kC) {
+              // block m = lane / 8: tokens 8 (n + m / 2).., channels 8 (m % 2)..
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  if (t + j >= bad) o[j] = __int_as_float(0x7FFFFFFF);
-              }
-              if (dv < a.Dv) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  if (t + j < n) row[(int64_t)(t + j) * a.o_st] = from_f<T>(o[j]);
+              for (int n = 0; n < 4; n += 2) {
+                const int row = cg * 32 + 8 * (n + (lane >> 4)) + (lane & 7);
+                stm4_t(stage_u + out_at<kRow>(row, hh * 2 + ((lane >> 3) & 1)), o[n][0], o[n][1], o[n + 1][0], o[n + 1][1]);
               }
             }
+            if (s_badany[cc & 3] == cc + 1)
+              spoil_outputs<kRow>(stage, s_bad + (cc & 3) * DV + wq * (DV / 4), cc);
+            __syncwarp();
+            constexpr int kRows = 32 / kVec;  // rows of a warp's store
+            const int v = lane % kVec, row0 = lane / kVec, dv = wq * (DV / 4) + v * 8;
+            T* dst = out + (x.t0 + c) * a.o_st + (int64_t)(x.h * G + g) * a.o_sh + wq * (DV / 4);
+            if (a.o_vec) {
+              dst += (int64_t)row0 * a.o_st + v * 8;
+              const int64_t step = (int64_t)kRows * a.o_st;
+              const int left = dv < a.Dv ? n_tok - row0 : 0;
+#pragma unroll
+              for (int z = 0; z < kC / kRows; ++z, dst += step)
+                if (z * kRows < left)
+                  *reinterpret_cast<uint4*>(dst) =
+                      *reinterpret_cast<const uint4*>(stage + out_at<kRow>(z * kRows + row0, v));
+            } else {
+              store_unaligned<T, kRow>(stage, dst, a.o_st, n_tok, a.Dv - wq * (DV / 4));
+            }
+            __syncwarp();
           }
         }
-        ++nu;
       }
     }
   } else {
-    // ------------------------------------------------------------ state
-    // Lane: channel dv as in the outputs, NC of the 64 dk columns of its group.
-    constexpr int NC = DV == 128 ? 64 : 32;
-    constexpr int NT = K::kStateWarps * 32;
-    const int sw = warp - K::kOutWarps, stid = threadIdx.x - K::kOutWarps * 32;
-    const int qd = sw & 3, cg = sw >> 2;
-    // the warp's TMEM lanes are those of its number modulo 4
-    const int dv = DV == 128 ? qd * 32 + lane : qd * 16 + (lane & 15);
-    const int c0 = cg * 64 + (DV == 128 ? 0 : (lane >> 4) * 32);
-    uint32_t cc = 0, ns = 0, nsync = 0;
+    // ------------------------------------------------------------ state and V'
+    // S: rows dv as in the outputs, columns dk = 64 cg + 8 n + fc and + 1.
     bool ok = true;
-    const uint32_t ta = tmem + ((uint32_t)(qd * 32) << 16) + K::kColKv + cg * 64;
-    float S[NC];
+    const int dv0 = wq * (DV / 4) + fr;
 
-    // all state warps meet (bounded, as every wait)
-    auto meet = [&]() -> bool {
-      warp_arrive(st_sync);
-      return warp_wait(st_sync, nsync++ & 1, ERR_SITE_DECAY_STATE, w);
+    // V' of chunk `chunk` (n tokens): v comes transposed from its tile (rows dv,
+    // tokens 8 m + fc and + 1), meets f (l^{n-1-j}), and goes out in parts.
+    auto factors = [&](float l2, int n, F2 (&f)[8]) {
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        const int d = n - 1 - 8 * m - fc;
+        f[m] = F2{d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1))};
+      }
     };
-    // S^T as two 16-bit parts in shared memory, for the product with the queries
-    auto put_s = [&](uint32_t chunk) -> bool {
-      if constexpr (OUT) {
-        float up = 1.f, undo = 1.f;
-        if constexpr (FP16) {
-          // the channel's largest entry sits in up to two warps and two half-warps
-          float m = 0.f;
-#pragma unroll
-          for (int j = 0; j < NC; ++j) m = fmaxf(m, fabsf(S[j]));
-          if (DV == 64) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-          float* mx = s_smax + (chunk & 1) * 256;
-          if (K::kCg > 1) {
-            mx[cg * 128 + dv] = m;
-            if (!meet()) return false;
-            m = fmaxf(mx[dv], mx[128 + dv]);
-          }
-          const int e = fp16_shift(m);
-          up = pow2i(e);
-          undo = pow2i(-e);
-        }
-        // the product with the S before it is done, so chunk - 2 has been put out
-        if (!warp_wait(s_empty, (ns & 1) ^ 1, ERR_SITE_DECAY_STATE, w)) return false;
-        if (FP16 && cg == 0) s_sscale[(chunk & 1) * 128 + dv] = undo;
-        uint8_t* base = sS + (c0 >> 6) * (DV * 128) + dv * 128;
-#pragma unroll
-        for (int ch = 0; ch < NC / 8; ++ch) {
-          uint32_t p[4][2];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) split2<T, 2>(S[ch * 8 + 2 * z] * up, S[ch * 8 + 2 * z + 1] * up, p[z]);
-          const int off = ((((c0 & 63) >> 3) + ch) ^ (dv & 7)) * 16;
-          *reinterpret_cast<uint4*>(base + off) = make_uint4(p[0][0], p[1][0], p[2][0], p[3][0]);
-          *reinterpret_cast<uint4*>(base + K::kSPart + off) = make_uint4(p[0][1], p[1][1], p[2][1], p[3][1]);
+    auto put_v = [&](uint32_t chunk, int n, const F2 (&f)[8]) -> bool {
+      const uint32_t st = chunk % K::kKvStages;
+      if (!warp_wait(&kv_full[st], (chunk / K::kKvStages) & 1, ERR_SITE_DECAY_V, w)) return false;
+      uint8_t* v = sV + st * K::kVBytes;
+      const uint32_t vu = smem_u32(v);
+      if (n < kC) {
+        // Tokens beyond the segment's end belong to others: zeros in their place,
+        // in k for KV and in v for V' and PV (each warp in its own channels of v).
+        uint8_t* k = sK + st * K::kKBytes;
+#pragma unroll 1
+        for (int e = wq * 32 + lane; e < K::kKBytes / 16; e += 128)
+          if (((e >> 3) & 63) >= n) *reinterpret_cast<uint4*>(k + e * 16) = make_uint4(0, 0, 0, 0);
+        constexpr int kV8 = DV / 32;  // vectors of a token in the warp's channels
+#pragma unroll 1
+        for (int e = n * kV8 + lane; e < kC * kV8; e += 32) {
+          const int j = e / kV8, d8 = wq * kV8 + e % kV8;
+          *reinterpret_cast<uint4*>(v + (d8 >> 3) * kTileBytes + j * 128 + (((d8 & 7) ^ (j & 7)) << 4)) =
+              make_uint4(0, 0, 0, 0);
         }
         fence_async_shared();
-        warp_arrive(s_full);
-        ++ns;
+        __syncwarp();
       }
-      return true;
-    };
-    // V' of chunk `chunk` (n tokens) into its buffer; returns fp16's power of two
-    auto put_v = [&](uint32_t chunk, int n, float l2, float& down) -> bool {
-      const uint32_t st = chunk % K::kKvStages;
-      if (!warp_wait(&kv_full[st], (chunk / K::kKvStages) & 1, ERR_SITE_DECAY_STATE, w)) return false;
-      uint8_t* v = sV + st * K::kVBytes;
-      uint8_t* dst = sVp + (chunk % VP) * K::kVParts * K::kVBytes;
-      constexpr int NV = K::kVBytes / 16 / NT;
-      if (n < kC) {
-        // tokens beyond the segment's end belong to others: zeros in their place
-        uint8_t* k = sK + st * K::kKBytes;
-        for (int e = stid; e < K::kKBytes / 16; e += NT)
-          if (((e >> 3) & 63) >= n) *reinterpret_cast<uint4*>(k + e * 16) = make_uint4(0, 0, 0, 0);
-      }
-      uint4 raw[NV];
-      uint32_t odd = 0, top = 0;
 #pragma unroll
-      for (int z = 0; z < NV; ++z) {
-        const int e = stid + z * NT, j = (e >> 3) & 63;
-        uint4 r = *reinterpret_cast<const uint4*>(v + e * 16);
-        if (j >= n) {
-          r = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(v + e * 16) = r;
-        }
-        raw[z] = r;
-        odd |= Half2<T>::non_finite(r.x) | Half2<T>::non_finite(r.y) | Half2<T>::non_finite(r.z) |
-               Half2<T>::non_finite(r.w);
+      for (int hh = 0; hh < NH; ++hh) {
+        const int d0 = wq * (DV / 4) + hh * 16;  // 16 channels
+        // block m = lane / 8 of a load: tokens 8 (2 z + m / 2).., channels d0 + 8 (m % 2)..
+        const int ch = ((d0 & 63) >> 3) + ((lane >> 3) & 1), tr = (lane & 7) + (lane >> 4) * 8;
+        const uint32_t at = vu + (d0 >> 6) * kTileBytes + tr * 128 + ((ch ^ (lane & 7)) << 4);
+        uint32_t raw[16];  // [token octet][row half]
+        uint32_t top = 0;  // largest magnitudes, as bits
+#pragma unroll
+        for (int z = 0; z < 4; ++z) ldm4_t(at + z * 2048, raw[4 * z], raw[4 * z + 1], raw[4 * z + 2], raw[4 * z + 3]);
+#pragma unroll
+        for (int y = 0; y < 16; y += 2)
+          top = __vimax3_u16x2(top, raw[y] & 0x7FFF7FFFu, raw[y + 1] & 0x7FFF7FFFu);
+        if (__any_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16) >= Half2<T>::kInf))
+          mark_non_finite<T>(v, d0, chunk, s_bad + (chunk & 3) * DV, &s_badany[chunk & 3]);
+        float up[2] = {1.f, 1.f};
         if constexpr (FP16) {
-          top = __vmaxu2(top, __vmaxu2(__vmaxu2(r.x & 0x7FFF7FFFu, r.y & 0x7FFF7FFFu),
-                                       __vmaxu2(r.z & 0x7FFF7FFFu, r.w & 0x7FFF7FFFu)));
-        }
-      }
-      if (odd) {
-        // An infinity or NaN in v: zero in its place for PV, where earlier tokens
-        // would meet it as 0 * inf; the O warps write NaN from its token on.
 #pragma unroll
-        for (int z = 0; z < NV; ++z) {
-          const int e = stid + z * NT, j = (e >> 3) & 63;
-          const int d0 = (e >> 9) * 64 + ((e & 7) ^ (j & 7)) * 8;
-          uint32_t q[4] = {raw[z].x, raw[z].y, raw[z].z, raw[z].w};
+          for (int r = 0; r < 2; ++r) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) m = __vmaxu2(m, raw[2 * y + r] & 0x7FFF7FFFu);
+            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            m = min(max(m & 0xFFFFu, m >> 16), 0x7BFFu);
+            const int e = fp16_shift(__half2float(__ushort_as_half((unsigned short)m)));
+            up[r] = pow2i(e);
+            if ((lane & 3) == 0) s_vscale[(chunk & 3) * 128 + d0 + fr + 8 * r] = pow2i(-e);
+          }
+        }
+        uint32_t part[K::kVParts][16];
+#pragma unroll
+        for (int h = 0; h < 16; h += 8) {
+          F2 g[8];
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
-            const uint32_t half = (q[y >> 1] >> (16 * (y & 1))) & 0xFFFFu;
-            if (Half2<T>::non_finite(half)) {
-              q[y >> 1] &= (y & 1) ? 0x0000FFFFu : 0xFFFF0000u;
-              atomicMax(&s_bad[(chunk % 3) * DV + d0 + y], ((chunk + 1) << 6) + (63 - j));
-              s_badany[chunk % 3] = chunk + 1;
-            }
+            g[y] = mul2(Half2<T>::unpack(raw[h + y]), f[(h + y) >> 1]);
+            if constexpr (FP16) g[y] = mul2(g[y], F2{up[y & 1], up[y & 1]});
           }
-          *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+#pragma unroll
+          for (int p = 0; p < K::kVParts; ++p)
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              part[p][h + y] = Half2<T>::pack(g[y].x, g[y].y);
+              if (p + 1 < K::kVParts) g[y] = sub2(g[y], Half2<T>::unpack(part[p][h + y]));
+            }
         }
-      }
-      float up = 1.f;
-      down = 1.f;
-      if constexpr (FP16) {
-        uint32_t m = max(top & 0xFFFFu, top >> 16);
-        m = __reduce_max_sync(0xffffffffu, m);
-        float* vm = s_vmax + (chunk & 1) * 8;
-        if (lane == 0) vm[sw] = __half2float(__ushort_as_half((unsigned short)min(m, 0x7BFFu)));
-        if (!meet()) return false;
-        float f = 0.f;
-#pragma unroll
-        for (int z = 0; z < K::kStateWarps; ++z) f = fmaxf(f, vm[z]);
-        const int e = fp16_shift(f);
-        up = pow2i(e);
-        down = pow2i(-e);
-      }
-#pragma unroll
-      for (int z = 0; z < NV; ++z) {
-        const int e = stid + z * NT, j = (e >> 3) & 63;
-        const float f = j < n ? exp2f(l2 * (float)(n - 1 - j)) * up : 0.f;
-        const uint32_t q[4] = {raw[z].x, raw[z].y, raw[z].z, raw[z].w};
-        uint32_t p[4][K::kVParts];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float2 g = Half2<T>::unpack(q[y]);
-          split2<T, K::kVParts>(g.x * f, g.y * f, p[y]);
+        // KV of the chunk before in this buffer has read its V'
+        if (hh == 0) {
+          if (!warp_wait(&ds_full[chunk % VP], ((chunk / VP) & 1) ^ 1, ERR_SITE_DECAY_V, w)) return false;
+          tc_fence_after();
         }
 #pragma unroll
-        for (int y = 0; y < K::kVParts; ++y)
-          *reinterpret_cast<uint4*>(dst + y * K::kVBytes + e * 16) = make_uint4(p[0][y], p[1][y], p[2][y], p[3][y]);
+        for (int q = 0; q < K::kVParts; ++q) {
+          if constexpr (TM) {
+            tmem_st_frag8(tlane + ((uint32_t)(hh * 16) << 16) + K::kColV + ((chunk % VP) * K::kVParts + q) * 32, part[q]);
+          } else {
+            const uint32_t to = smem_u32(sVp) + q * K::kVBytes + (at - vu);
+#pragma unroll
+            for (int z = 0; z < 4; ++z)
+              stm4_t(to + z * 2048, part[q][4 * z], part[q][4 * z + 1], part[q][4 * z + 2], part[q][4 * z + 3]);
+          }
+        }
       }
-      fence_async_shared();
+      if constexpr (TM) {
+        tmem_st_wait();
+        tc_fence_before();
+      } else {
+        fence_async_shared();
+      }
       warp_arrive(&vp_full[chunk % VP]);
       return true;
     };
 
-    for (int64_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
-      Unit x;
-      if (!get_unit<OUT>(a, u, x)) continue;
-      const float ld = a.log_decay[x.h];
-      const float l2 = log2_decay(ld);
-      const int64_t at = (int64_t)c0 * a.Dv + dv;
+    if (TM && wg == K::kV) {
+      uint32_t cc = 0;
+      for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
+        Unit x;
+        if (!get_unit<OUT>(a, u, x)) continue;
+        const float l2 = log2_decay(a.log_decay[x.h]);
+        F2 f[8];
+        for (int c = 0; c < x.len && ok; c += kC, ++cc) {
+          const int n = min(kC, x.len - c);
+          if (c == 0 || n < kC) factors(l2, n, f);
+          ok = put_v(cc, n, f);
+        }
+      }
+    } else {
+      if constexpr (K::kMove) regs_up<K::kRegS>();
+      uint32_t cc = 0, ns = 0;
+      float S[NH][K::kCg][32];
+      for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
+        Unit x;
+        if (!get_unit<OUT>(a, u, x)) continue;
+        const float ld = a.log_decay[x.h], l2 = log2_decay(ld);
+        const float2 whole = pow_hi_lo(ld, kC), tail = pow_hi_lo(ld, x.len & (kC - 1));
+        const int64_t at = (int64_t)fc * a.Dv + dv0;
 #pragma unroll
-      for (int j = 0; j < NC; ++j)
-        S[j] = (x.start && dv < a.Dv && c0 + j < a.Dk) ? x.start[at + (int64_t)j * a.Dv] : 0.f;
-      if (x.len > 0) {
-        if (x.start && !(ok = put_s(cc))) break;
-        float2 dec = pow_hi_lo(ld, min(kC, x.len));
-        float down = 1.f, next = 1.f;  // fp16's power of two of this chunk's V' and the next's
-        if (VP == 2 && !(ok = put_v(cc, min(kC, x.len), l2, next))) break;
+        for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+          for (int cg = 0; cg < K::kCg; ++cg)
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+              const bool in = x.start && cg * 64 + m * 8 < a.Dk;
+              const float* src = x.start + at + (cg * 64 + m * 8) * a.Dv;
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const bool on = in && dv0 + hh * 16 + r * 8 < a.Dv;
+                S[hh][cg][4 * m + 2 * r] = on ? src[hh * 16 + r * 8] : 0.f;
+                S[hh][cg][4 * m + 2 * r + 1] = on ? src[a.Dv + hh * 16 + r * 8] : 0.f;
+              }
+            }
+        F2 f[8];
         for (int c = 0; c < x.len; c += kC, ++cc) {
           const int n = min(kC, x.len - c);
-          if (n < kC && c > 0) dec = pow_hi_lo(ld, n);
-          if (VP == 1) {
-            if (!(ok = put_v(cc, n, l2, down))) break;
-          } else {
-            down = next;
-            if (c + kC < x.len && !(ok = put_v(cc + 1, min(kC, x.len - c - kC), l2, next))) break;
+          if (OUT && (c > 0 || x.start)) {
+            // S^T in 16 bits, for the product with the queries; the one before it
+            // is done when s_empty comes round
+            if (!(ok = warp_wait(s_empty, (ns & 1) ^ 1, ERR_SITE_DECAY_STATE, w))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int hh = 0; hh < NH; ++hh) {
+              float up[2] = {1.f, 1.f};
+              if constexpr (FP16) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  float m = 0.f;
+#pragma unroll
+                  for (int cg = 0; cg < K::kCg; ++cg)
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                      m = fmaxf(m, fmaxf(fabsf(S[hh][cg][4 * y + 2 * r]), fabsf(S[hh][cg][4 * y + 2 * r + 1])));
+                  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                  const int e = fp16_shift(m);
+                  up[r] = pow2i(e);
+                  if ((lane & 3) == 0) s_sscale[(cc & 1) * 128 + dv0 + hh * 16 + 8 * r] = pow2i(-e);
+                }
+              }
+#pragma unroll
+              for (int cg = 0; cg < K::kCg; ++cg) {
+                uint32_t p[16];
+#pragma unroll
+                for (int y = 0; y < 16; ++y) {
+                  F2 z{S[hh][cg][2 * y], S[hh][cg][2 * y + 1]};
+                  if constexpr (FP16) z = mul2(z, F2{up[y & 1], up[y & 1]});
+                  p[y] = Half2<T>::pack(z.x, z.y);
+                }
+                if constexpr (TM) {
+                  tmem_st_frag8(tlane + ((uint32_t)(hh * 16) << 16) + K::kColS + cg * 32, p);
+                } else {
+                  // block m = lane / 8: rows dv + 8 (m % 2).., columns 8 (m / 2)..
+                  const int row = wq * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+                  const uint32_t to = smem_u32(sS) + cg * (DV * 128) + row * 128;
+#pragma unroll
+                  for (int z = 0; z < 4; ++z)
+                    stm4(to + (((2 * z + (lane >> 4)) ^ (row & 7)) << 4), p[4 * z], p[4 * z + 1], p[4 * z + 2],
+                         p[4 * z + 3]);
+                }
+              }
+            }
+            if constexpr (TM) {
+              tmem_st_wait();
+              tc_fence_before();
+            } else {
+              fence_async_shared();
+            }
+            warp_arrive(s_full);
+            ++ns;
+          }
+          if constexpr (!TM) {
+            if (c == 0 || n < kC) factors(l2, n, f);
+            if (!(ok = put_v(cc, n, f))) break;
           }
           if (!(ok = warp_wait(&ds_full[cc % VP], (cc / VP) & 1, ERR_SITE_DECAY_STATE, w))) break;
           tc_fence_after();
+          const float2 dec = n == kC ? whole : tail;
+          const F2 hi{dec.x, dec.x}, lo{dec.y, dec.y};
+          constexpr int NQ = NH * 2 * K::kCg;  // groups of 16 rows x 32 columns, one load ahead
+          const uint32_t ta = tlane + K::kColKv + (cc % VP) * DK;
+          auto group = [&](int q) { return ta + ((uint32_t)(q / (2 * K::kCg) * 16) << 16) + q % (2 * K::kCg) * 32; };
+          float r[2][16];
+          tmem_ld_frag4(group(0), r[0]);
 #pragma unroll
-          for (int b = 0; b < NC / 16; ++b) {
-            float r[16];
-            tmem_ld16<DV>(ta + (cc % VP) * DK + b * 16, r);
+          for (int q = 0; q < NQ; ++q) {
+            tmem_wait16(r[q & 1]);
+            if (q + 1 < NQ) {
+              tmem_ld_frag4(group(q + 1), r[(q + 1) & 1]);
+            } else {
+              tc_fence_before();
+              warp_arrive(&ds_empty[cc % VP]);
+            }
+            const int hh = q / (2 * K::kCg);
+            float dn[2] = {1.f, 1.f};
+            if constexpr (FP16) {
+              dn[0] = s_vscale[(cc & 3) * 128 + dv0 + hh * 16];
+              dn[1] = s_vscale[(cc & 3) * 128 + dv0 + hh * 16 + 8];
+            }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float& s = S[b * 16 + j];
-              const float add = FP16 ? r[j] * down : r[j];
-              s = fmaf(dec.x, s, fmaf(dec.y, s, add));
+            for (int y = 0; y < 8; ++y) {
+              F2 add{r[q & 1][2 * y], r[q & 1][2 * y + 1]};
+              if constexpr (FP16) add = mul2(add, F2{dn[y & 1], dn[y & 1]});
+              float* e = &S[hh][q / 2 % K::kCg][(q & 1) * 16 + 2 * y];
+              const F2 z = fma2(hi, F2{e[0], e[1]}, fma2(lo, F2{e[0], e[1]}, add));
+              e[0] = z.x;
+              e[1] = z.y;
             }
           }
-          tc_fence_before();
-          if (OUT && c + kC < x.len && !(ok = put_s(cc + 1))) break;
         }
         if (!ok) break;
-      }
-      if (x.end && dv < a.Dv) {
+        if (x.end) {
 #pragma unroll
-        for (int j = 0; j < NC; ++j)
-          if (c0 + j < a.Dk) x.end[at + (int64_t)j * a.Dv] = S[j];
+          for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+            for (int cg = 0; cg < K::kCg; ++cg)
+#pragma unroll
+              for (int m = 0; m < 8; ++m) {
+                if (cg * 64 + m * 8 >= a.Dk) continue;
+                float* dst = x.end + at + (cg * 64 + m * 8) * a.Dv;
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                  if (dv0 + hh * 16 + r * 8 < a.Dv) {
+                    dst[hh * 16 + r * 8] = S[hh][cg][4 * m + 2 * r];
+                    dst[a.Dv + hh * 16 + r * 8] = S[hh][cg][4 * m + 2 * r + 1];
+                  }
+              }
+        }
       }
     }
   }

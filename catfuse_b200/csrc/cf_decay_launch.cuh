@@ -26,8 +26,8 @@ int launch_one(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
     if (dev >= 0 && dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
-  const int64_t most = (int64_t)sms * C::kCtas;
-  cfg.gridDim = dim3((unsigned)(a.n_units < most ? a.n_units : most));
+  const unsigned most = (unsigned)(sms * C::kCtas);
+  cfg.gridDim = dim3(a.n_units < most ? a.n_units : most);
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
