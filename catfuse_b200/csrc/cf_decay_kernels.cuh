@@ -93,19 +93,21 @@ struct Wait {
   volatile int* abort;
 };
 
-// A whole warp waits (uniform result).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t site, const Wait& w) {
+// A whole warp waits (uniform result).  False: the limit ran out, or another role
+// gave up; the role then leaves its loop and reports its site (give_up).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Wait& w) {
+  uint32_t i = w.max_polls;
 #pragma unroll 1
-  for (uint32_t i = 0; i < w.max_polls; ++i) {
+  do {
     if (__any_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    if ((i & 255u) == 255u && __any_sync(0xffffffffu, *w.abort != 0)) return false;
-  }
-  if ((threadIdx.x & 31) == 0) {
+  } while (--i && !__any_sync(0xffffffffu, *w.abort != 0));
+  return false;
+}
+__device__ __forceinline__ void give_up(int32_t site, const Wait& w) {
+  if ((threadIdx.x & 31) == 0 && !*w.abort) {
     atomicCAS(w.err, 0, site);
     *w.abort = 1;
   }
-  __syncwarp();
-  return false;
 }
 __device__ __forceinline__ bool warp_test(uint64_t* bar, uint32_t parity) {
   return __any_sync(0xffffffffu, mbar_test_wait(bar, parity));
@@ -238,31 +240,27 @@ __device__ __forceinline__ void mma_commit(uint32_t one, uint64_t* bar) {
       : "memory");
 }
 
-// Two fp32 values at a time.
-struct alignas(8) F2 {
-  float x, y;
-};
-__device__ __forceinline__ uint64_t f2_bits(F2 a) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+// Two fp32 values at a time, in a register pair.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 pack2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
   return r;
 }
-__device__ __forceinline__ F2 f2_from(uint64_t r) {
-  F2 a;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
-  return a;
+__device__ __forceinline__ void unpack2(F2 a, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a));
 }
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return f2_from(r);
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
-  return f2_from(r);
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
-__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, F2{-1.f, -1.f}, a); }
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, pack2(-1.f, -1.f), a); }
 
 // Registers move between warpgroups: the sum stays within the launch's share.
 template <int N>
@@ -297,24 +295,28 @@ template <typename T>
 struct Half2;
 template <>
 struct Half2<__half> {
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+  static __device__ __forceinline__ uint32_t pack(F2 v) {
+    float a, b;
+    unpack2(v, a, b);
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ F2 unpack(uint32_t u) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
-    return F2{f.x, f.y};
+    return pack2(f.x, f.y);
   }
   static constexpr uint32_t kInf = 0x7C00;
 };
 template <>
 struct Half2<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+  static __device__ __forceinline__ uint32_t pack(F2 v) {
+    float a, b;
+    unpack2(v, a, b);
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ F2 unpack(uint32_t u) {
-    return F2{__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)};
+    return pack2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   }
   static constexpr uint32_t kInf = 0x7F80;
 };
@@ -324,7 +326,7 @@ template <typename T, int PARTS>
 __device__ __forceinline__ void split2(F2 a, uint32_t (&out)[PARTS]) {
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) {
-    out[p] = Half2<T>::pack(a.x, a.y);
+    out[p] = Half2<T>::pack(a);
     if (p + 1 < PARTS) a = sub2(a, Half2<T>::unpack(out[p]));
   }
 }
@@ -446,15 +448,15 @@ __device__ __forceinline__ bool get_unit(const DecayArgs& a, uint32_t u, Unit& x
   return true;
 }
 
-// The infinities and NaN among 16 channels of a tile of v: zeros in their place,
+// The infinities and NaN among n channels of a tile of v: zeros in their place,
 // where PV would meet them as 0 * inf for earlier tokens; the O warps write NaN
 // from their token on.
 template <typename T>
-__device__ __forceinline__ void mark_non_finite(uint8_t* v, int d0, uint32_t chunk, uint32_t* bad,
-                                             volatile uint32_t* any) {
+__device__ __forceinline__ void mark_non_finite(uint8_t* v, int d0, int n, uint32_t chunk, uint32_t* bad,
+                                                volatile uint32_t* any) {
 #pragma unroll 1
-  for (int e = threadIdx.x & 31; e < kC * 16; e += 32) {
-    const int j = e >> 4, d = d0 + (e & 15);
+  for (int e = threadIdx.x & 31; e < kC * n; e += 32) {
+    const int j = e / n, d = d0 + e % n;
     uint16_t* at = reinterpret_cast<uint16_t*>(v + (d >> 6) * kTileBytes + j * 128 +
                                                ((((d & 63) >> 3) ^ (j & 7)) << 4) + (d & 7) * 2);
     if ((*at & 0x7FFFu) >= Half2<T>::kInf) {
@@ -603,7 +605,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         if (!get_unit<OUT>(a, u, x)) continue;
         for (int c = 0; c < x.len && ok; c += kC, ++cc) {
           const int st = cc % K::kKvStages;
-          if (!(ok = warp_wait(&kv_empty[st], ((cc / K::kKvStages) & 1) ^ 1, ERR_SITE_DECAY_LOAD, w))) break;
+          if (!(ok = warp_wait(&kv_empty[st], ((cc / K::kKvStages) & 1) ^ 1, w))) break;
           const int t = (int)(x.t0 + c);
           if (lane == 0 && !drop) {
             mbar_arrive_expect_tx(&kv_full[st], K::kKBytes + K::kVBytes);
@@ -620,7 +622,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           if constexpr (OUT) {
             for (int g = 0; g < G; ++g, ++it) {
               const int qs = it % K::kQStages;
-              if (!(ok = warp_wait(&q_empty[qs], ((it / K::kQStages) & 1) ^ 1, ERR_SITE_DECAY_LOAD, w))) break;
+              if (!(ok = warp_wait(&q_empty[qs], ((it / K::kQStages) & 1) ^ 1, w))) break;
               if (lane == 0) {
                 mbar_arrive_expect_tx(&q_full[qs], K::kKBytes);
                 for (int p = 0; p < DK / 64; p += a.qp)
@@ -634,6 +636,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         }
       }
       if (!ok) {
+        give_up(ERR_SITE_DECAY_LOAD, w);
         // the loads in flight land before the CTA ends
         for (int s = 0; s < 4; ++s) {
           for (uint32_t i = 0; (kv_used >> (2 * s) & 2u) && i < (1u << 16); ++i)
@@ -664,7 +667,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       bool ok = true, qk_early = false;
       auto issue_qk = [&](uint32_t qs, uint32_t st) {
         const uint64_t ad = dQ + (uint64_t)(qs * (K::kKBytes >> 4)), bd = dKk + (uint64_t)(st * (K::kKBytes >> 4));
-#pragma unroll
+#pragma unroll 1
         for (int p = 0; p < DK / 64; ++p)
 #pragma unroll
           for (int s = 0; s < 4; ++s)
@@ -678,25 +681,25 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         for (int c = 0; c < len && ok; c += kC, ++cc) {
           const uint32_t st = cc % K::kKvStages;
           const uint32_t vb = cc % VP;
-          if (!(ok = warp_wait(&kv_full[st], (cc / K::kKvStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
+          if (!(ok = warp_wait(&kv_full[st], (cc / K::kKvStages) & 1, w))) break;
           if constexpr (OUT) {
             if (!qk_early) {
               const uint32_t qs = it % K::kQStages;
-              if (!(ok = warp_wait(&q_full[qs], (it / K::kQStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
+              if (!(ok = warp_wait(&q_full[qs], (it / K::kQStages) & 1, w))) break;
               tc_fence_after();
               issue_qk(qs, st);
             }
             qk_early = false;
           }
-          if (!(ok = warp_wait(&vp_full[vb], (cc / VP) & 1, ERR_SITE_DECAY_MMA, w))) break;
-          if (!(ok = warp_wait(&ds_empty[vb], ((cc / VP) & 1) ^ 1, ERR_SITE_DECAY_MMA, w))) break;
+          if (!(ok = warp_wait(&vp_full[vb], (cc / VP) & 1, w))) break;
+          if (!(ok = warp_wait(&ds_empty[vb], ((cc / VP) & 1) ^ 1, w))) break;
           tc_fence_after();
           {
             const uint64_t ad = dVpm + (uint64_t)(vb * K::kVParts * (K::kVBytes >> 4));
             const uint32_t at = tm + K::kColV + vb * K::kVParts * 32;
             const uint64_t bd = dKm + (uint64_t)(st * (K::kKBytes >> 4));
             const uint32_t d = tm + K::kColKv + vb * DK;
-#pragma unroll
+#pragma unroll 1
             for (int p = K::kVParts - 1; p >= 0; --p)  // the small parts first
 #pragma unroll
               for (int s = 0; s < 4; ++s) {
@@ -712,8 +715,8 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             const bool has_s = c > 0 || started;
             for (int g = 0; g < G; ++g, ++it) {
               const uint32_t qs = it % K::kQStages;
-              if (!(ok = warp_wait(p_full, it & 1, ERR_SITE_DECAY_MMA, w))) break;
-              if (!(ok = warp_wait(o_empty, (it & 1) ^ 1, ERR_SITE_DECAY_MMA, w))) break;
+              if (!(ok = warp_wait(p_full, it & 1, w))) break;
+              if (!(ok = warp_wait(o_empty, (it & 1) ^ 1, w))) break;
               tc_fence_after();
               {
                 const uint64_t ad = dVm + (uint64_t)(st * (K::kVBytes >> 4));
@@ -726,7 +729,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
               const bool same = g + 1 < G;
               const uint32_t nq = (it + 1) % K::kQStages;
               const uint32_t nst = same ? st : (cc + 1) % K::kKvStages;
-              if (same && !(ok = warp_wait(&q_full[nq], ((it + 1) / K::kQStages) & 1, ERR_SITE_DECAY_MMA, w))) break;
+              if (same && !(ok = warp_wait(&q_full[nq], ((it + 1) / K::kQStages) & 1, w))) break;
               if (same || (c + kC < len && warp_test(&q_full[nq], ((it + 1) / K::kQStages) & 1) &&
                            warp_test(&kv_full[nst], ((cc + 1) / K::kKvStages) & 1))) {
                 issue_qk(nq, nst);
@@ -734,10 +737,10 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
               }
               if (!same) mma_commit(one, &kv_empty[st]);
               if (has_s) {
-                if (g == 0 && !(ok = warp_wait(s_full, ns & 1, ERR_SITE_DECAY_MMA, w))) break;
+                if (g == 0 && !(ok = warp_wait(s_full, ns & 1, w))) break;
                 tc_fence_after();
                 const uint64_t bd = dQ + (uint64_t)(qs * (K::kKBytes >> 4));
-#pragma unroll
+#pragma unroll 1
                 for (int p = 0; p < DK / 64; ++p)
 #pragma unroll
                   for (int s = 0; s < 4; ++s) {
@@ -756,6 +759,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           }
         }
       }
+      if (!ok) give_up(ERR_SITE_DECAY_MMA, w);
       mma_commit(one, done_bar);
       for (uint32_t p = 0; p < kMaxPolls; ++p)
         if (mbar_try_wait(done_bar, 0)) break;
@@ -784,11 +788,11 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int d = i + 8 * r - 8 * n - fc;
-            f[n][r] = F2{d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1))};
+            f[n][r] = pack2(d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1)));
           }
         const int items = (x.len + kC - 1) / kC * G;
         for (int k = 0; k < items; ++k, ++it) {
-          if (!(ok = warp_wait(qk_full, it & 1, ERR_SITE_DECAY_P, w))) break;
+          if (!(ok = warp_wait(qk_full, it & 1, w))) break;
           tc_fence_after();
           float q[32];
           tmem_ld_frag8(tlane, q);
@@ -797,9 +801,8 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const F2 y = mul2(F2{q[4 * n + 2 * r], q[4 * n + 2 * r + 1]}, f[n][r]);
-              q[4 * n + 2 * r] = y.x;
-              q[4 * n + 2 * r + 1] = y.y;
+              const F2 y = mul2(pack2(q[4 * n + 2 * r], q[4 * n + 2 * r + 1]), f[n][r]);
+              unpack2(y, q[4 * n + 2 * r], q[4 * n + 2 * r + 1]);
               // above the diagonal 0 * inf must not appear
               if (i - fc < 8 * n - 8 * r) q[4 * n + 2 * r] = 0.f;
               if (i - fc < 8 * n - 8 * r + 1) q[4 * n + 2 * r + 1] = 0.f;
@@ -824,7 +827,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             }
           }
           // PV of the item before has read P
-          if (!(ok = warp_wait(p_empty, (it & 1) ^ 1, ERR_SITE_DECAY_P, w))) break;
+          if (!(ok = warp_wait(p_empty, (it & 1) ^ 1, w))) break;
           if (FP16 && (lane & 3) == 0) {
             s_pscale[(it & 1) * 64 + i] = undo[0];
             s_pscale[(it & 1) * 64 + i + 8] = undo[1];
@@ -833,13 +836,14 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           for (int n = 0; n < 8; n += 2) {
             uint32_t p[4];
 #pragma unroll
-            for (int z = 0; z < 4; ++z) p[z] = Half2<T>::pack(q[4 * n + 2 * z], q[4 * n + 2 * z + 1]);
+            for (int z = 0; z < 4; ++z) p[z] = Half2<T>::pack(pack2(q[4 * n + 2 * z], q[4 * n + 2 * z + 1]));
             stm4(prow + (((n + (lane >> 4)) ^ (si & 7)) << 4), p[0], p[1], p[2], p[3]);
           }
           fence_async_shared();
           warp_arrive(p_full);
         }
       }
+      if (!ok) give_up(ERR_SITE_DECAY_P, w);
     }
   } else if (OUT && wg == K::kO) {
     // ------------------------------------------------------------ outputs
@@ -860,58 +864,60 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         F2 grow[8];  // scale l^{i+1}
 #pragma unroll
         for (int n = 0; n < 8; ++n)
-          grow[n] = F2{a.scale * exp2_fast(l2 * (float)(8 * n + fc + 1)), a.scale * exp2_fast(l2 * (float)(8 * n + fc + 2))};
+          grow[n] = pack2(a.scale * exp2_fast(l2 * (float)(8 * n + fc + 1)),
+                          a.scale * exp2_fast(l2 * (float)(8 * n + fc + 2)));
         for (int c = 0; c < x.len && ok; c += kC, ++cc) {
           const bool has_s = c > 0 || x.start != nullptr;
           const int n_tok = min(kC, x.len - c);
           for (int g = 0; g < G; ++g, ++it) {
-            if (!(ok = warp_wait(o_full, it & 1, ERR_SITE_DECAY_O, w))) break;
+            if (!(ok = warp_wait(o_full, it & 1, w))) break;
             tc_fence_after();
             // groups of 16 channels x 32 tokens, one load ahead
-            auto group = [&](int q) { return tlane + ((uint32_t)(q / 2 * 16) << 16) + q % 2 * 32; };
             float p[2][16], z[2][16];
-            tmem_ld_frag4(group(0) + K::kColOp, p[0]);
-            tmem_ld_frag4(group(0) + K::kColOs, z[0]);
-#pragma unroll
-            for (int q = 0; q < 2 * NH; ++q) {
-              const int hh = q / 2, cg = q % 2, b = q & 1;
-              tmem_wait16(p[b]);
-              tmem_wait16(z[b]);
-              if (q + 1 < 2 * NH) {
-                tmem_ld_frag4(group(q + 1) + K::kColOp, p[b ^ 1]);
-                tmem_ld_frag4(group(q + 1) + K::kColOs, z[b ^ 1]);
-              }
+            tmem_ld_frag4(tlane + K::kColOp, p[0]);
+            tmem_ld_frag4(tlane + K::kColOs, z[0]);
+#pragma unroll 1
+            for (int hh = 0; hh < NH; ++hh) {
               float ss[2] = {1.f, 1.f};
               if constexpr (FP16) {
                 ss[0] = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr];
                 ss[1] = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr + 8];
               }
-              uint32_t o[4][2];
 #pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                F2 pf = F2{a.scale, a.scale};
-                if constexpr (FP16) {
-                  const F2 ps = *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + cg * 32 + 8 * n + fc]);
-                  pf = mul2(pf, ps);
+              for (int cg = 0; cg < 2; ++cg) {
+                tmem_wait16(p[cg]);
+                tmem_wait16(z[cg]);
+                if (cg == 0 || hh + 1 < NH) {
+                  const uint32_t ta = tlane + ((uint32_t)((hh + cg) * 16) << 16) + (cg == 0 ? 32 : 0);
+                  tmem_ld_frag4(ta + K::kColOp, p[cg ^ 1]);
+                  tmem_ld_frag4(ta + K::kColOs, z[cg ^ 1]);
                 }
+                uint32_t o[4][2];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                  F2 y = mul2(F2{p[b][4 * n + 2 * r], p[b][4 * n + 2 * r + 1]}, pf);
-                  F2 x2 = F2{z[b][4 * n + 2 * r], z[b][4 * n + 2 * r + 1]};
-                  if constexpr (FP16) x2 = mul2(x2, F2{ss[r], ss[r]});
-                  if (has_s) y = fma2(grow[cg * 4 + n], x2, y);
-                  o[n][r] = Half2<T>::pack(y.x, y.y);
+                for (int n = 0; n < 4; ++n) {
+                  F2 pf = pack2(a.scale, a.scale);
+                  if constexpr (FP16)
+                    pf = mul2(pf, *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + cg * 32 + 8 * n + fc]));
+#pragma unroll
+                  for (int r = 0; r < 2; ++r) {
+                    F2 y = mul2(pack2(p[cg][4 * n + 2 * r], p[cg][4 * n + 2 * r + 1]), pf);
+                    F2 x2 = pack2(z[cg][4 * n + 2 * r], z[cg][4 * n + 2 * r + 1]);
+                    if constexpr (FP16) x2 = mul2(x2, pack2(ss[r], ss[r]));
+                    if (has_s) y = fma2(grow[cg * 4 + n], x2, y);
+                    o[n][r] = Half2<T>::pack(y);
+                  }
                 }
-              }
-              if (q == 2 * NH - 1) {  // accumulators and scales are read
-                tc_fence_before();
-                warp_arrive(o_empty);
-              }
-              // block m = lane / 8: tokens 8 (n + m / 2).., channels 8 (m % 2)..
+                if (hh == NH - 1 && cg == 1) {  // accumulators and scales are read
+                  tc_fence_before();
+                  warp_arrive(o_empty);
+                }
+                // block m = lane / 8: tokens 8 (n + m / 2).., channels 8 (m % 2)..
 #pragma unroll
-              for (int n = 0; n < 4; n += 2) {
-                const int row = cg * 32 + 8 * (n + (lane >> 4)) + (lane & 7);
-                stm4_t(stage_u + out_at<kRow>(row, hh * 2 + ((lane >> 3) & 1)), o[n][0], o[n][1], o[n + 1][0], o[n + 1][1]);
+                for (int n = 0; n < 4; n += 2) {
+                  const int row = cg * 32 + 8 * (n + (lane >> 4)) + (lane & 7);
+                  stm4_t(stage_u + out_at<kRow>(row, hh * 2 + ((lane >> 3) & 1)), o[n][0], o[n][1], o[n + 1][0],
+                         o[n + 1][1]);
+                }
               }
             }
             if (s_badany[cc & 3] == cc + 1)
@@ -936,6 +942,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           }
         }
       }
+      if (!ok) give_up(ERR_SITE_DECAY_O, w);
     }
   } else {
     // ------------------------------------------------------------ state and V'
@@ -949,12 +956,12 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 #pragma unroll
       for (int m = 0; m < 8; ++m) {
         const int d = n - 1 - 8 * m - fc;
-        f[m] = F2{d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1))};
+        f[m] = pack2(d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1)));
       }
     };
     auto put_v = [&](uint32_t chunk, int n, const F2 (&f)[8]) -> bool {
       const uint32_t st = chunk % K::kKvStages;
-      if (!warp_wait(&kv_full[st], (chunk / K::kKvStages) & 1, ERR_SITE_DECAY_V, w)) return false;
+      if (!warp_wait(&kv_full[st], (chunk / K::kKvStages) & 1, w)) return false;
       uint8_t* v = sV + st * K::kVBytes;
       const uint32_t vu = smem_u32(v);
       if (n < kC) {
@@ -974,7 +981,8 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         fence_async_shared();
         __syncwarp();
       }
-#pragma unroll
+      bool odd = false;
+#pragma unroll 1
       for (int hh = 0; hh < NH; ++hh) {
         const int d0 = wq * (DV / 4) + hh * 16;  // 16 channels
         // block m = lane / 8 of a load: tokens 8 (2 z + m / 2).., channels d0 + 8 (m % 2)..
@@ -987,8 +995,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 #pragma unroll
         for (int y = 0; y < 16; y += 2)
           top = __vimax3_u16x2(top, raw[y] & 0x7FFF7FFFu, raw[y + 1] & 0x7FFF7FFFu);
-        if (__any_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16) >= Half2<T>::kInf))
-          mark_non_finite<T>(v, d0, chunk, s_bad + (chunk & 3) * DV, &s_badany[chunk & 3]);
+        odd = odd || max(top & 0xFFFFu, top >> 16) >= Half2<T>::kInf;
         float up[2] = {1.f, 1.f};
         if constexpr (FP16) {
 #pragma unroll
@@ -1011,19 +1018,19 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             g[y] = mul2(Half2<T>::unpack(raw[h + y]), f[(h + y) >> 1]);
-            if constexpr (FP16) g[y] = mul2(g[y], F2{up[y & 1], up[y & 1]});
+            if constexpr (FP16) g[y] = mul2(g[y], pack2(up[y & 1], up[y & 1]));
           }
 #pragma unroll
           for (int p = 0; p < K::kVParts; ++p)
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
-              part[p][h + y] = Half2<T>::pack(g[y].x, g[y].y);
+              part[p][h + y] = Half2<T>::pack(g[y]);
               if (p + 1 < K::kVParts) g[y] = sub2(g[y], Half2<T>::unpack(part[p][h + y]));
             }
         }
         // KV of the chunk before in this buffer has read its V'
         if (hh == 0) {
-          if (!warp_wait(&ds_full[chunk % VP], ((chunk / VP) & 1) ^ 1, ERR_SITE_DECAY_V, w)) return false;
+          if (!warp_wait(&ds_full[chunk % VP], ((chunk / VP) & 1) ^ 1, w)) return false;
           tc_fence_after();
         }
 #pragma unroll
@@ -1038,6 +1045,8 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           }
         }
       }
+      if (__any_sync(0xffffffffu, odd))
+        mark_non_finite<T>(v, wq * (DV / 4), DV / 4, chunk, s_bad + (chunk & 3) * DV, &s_badany[chunk & 3]);
       if constexpr (TM) {
         tmem_st_wait();
         tc_fence_before();
@@ -1064,7 +1073,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
     } else {
       if constexpr (K::kMove) regs_up<K::kRegS>();
       uint32_t cc = 0, ns = 0;
-      float S[NH][K::kCg][32];
+      F2 S[NH][K::kCg][16];  // pair y of 64 columns: octet y / 2, row half y % 2
       for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
         if (!get_unit<OUT>(a, u, x)) continue;
@@ -1082,8 +1091,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 const bool on = in && dv0 + hh * 16 + r * 8 < a.Dv;
-                S[hh][cg][4 * m + 2 * r] = on ? src[hh * 16 + r * 8] : 0.f;
-                S[hh][cg][4 * m + 2 * r + 1] = on ? src[a.Dv + hh * 16 + r * 8] : 0.f;
+                S[hh][cg][2 * m + r] = on ? pack2(src[hh * 16 + r * 8], src[a.Dv + hh * 16 + r * 8]) : 0;
               }
             }
         F2 f[8];
@@ -1092,7 +1100,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           if (OUT && (c > 0 || x.start)) {
             // S^T in 16 bits, for the product with the queries; the one before it
             // is done when s_empty comes round
-            if (!(ok = warp_wait(s_empty, (ns & 1) ^ 1, ERR_SITE_DECAY_STATE, w))) break;
+            if (!(ok = warp_wait(s_empty, (ns & 1) ^ 1, w))) break;
             tc_fence_after();
 #pragma unroll
             for (int hh = 0; hh < NH; ++hh) {
@@ -1104,8 +1112,11 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 #pragma unroll
                   for (int cg = 0; cg < K::kCg; ++cg)
 #pragma unroll
-                    for (int y = 0; y < 8; ++y)
-                      m = fmaxf(m, fmaxf(fabsf(S[hh][cg][4 * y + 2 * r]), fabsf(S[hh][cg][4 * y + 2 * r + 1])));
+                    for (int y = 0; y < 8; ++y) {
+                      float e, g;
+                      unpack2(S[hh][cg][2 * y + r], e, g);
+                      m = fmaxf(m, fmaxf(fabsf(e), fabsf(g)));
+                    }
                   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                   const int e = fp16_shift(m);
@@ -1118,9 +1129,9 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
                 uint32_t p[16];
 #pragma unroll
                 for (int y = 0; y < 16; ++y) {
-                  F2 z{S[hh][cg][2 * y], S[hh][cg][2 * y + 1]};
-                  if constexpr (FP16) z = mul2(z, F2{up[y & 1], up[y & 1]});
-                  p[y] = Half2<T>::pack(z.x, z.y);
+                  F2 z = S[hh][cg][y];
+                  if constexpr (FP16) z = mul2(z, pack2(up[y & 1], up[y & 1]));
+                  p[y] = Half2<T>::pack(z);
                 }
                 if constexpr (TM) {
                   tmem_st_frag8(tlane + ((uint32_t)(hh * 16) << 16) + K::kColS + cg * 32, p);
@@ -1148,10 +1159,10 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             if (c == 0 || n < kC) factors(l2, n, f);
             if (!(ok = put_v(cc, n, f))) break;
           }
-          if (!(ok = warp_wait(&ds_full[cc % VP], (cc / VP) & 1, ERR_SITE_DECAY_STATE, w))) break;
+          if (!(ok = warp_wait(&ds_full[cc % VP], (cc / VP) & 1, w))) break;
           tc_fence_after();
           const float2 dec = n == kC ? whole : tail;
-          const F2 hi{dec.x, dec.x}, lo{dec.y, dec.y};
+          const F2 hi = pack2(dec.x, dec.x), lo = pack2(dec.y, dec.y);
           constexpr int NQ = NH * 2 * K::kCg;  // groups of 16 rows x 32 columns, one load ahead
           const uint32_t ta = tlane + K::kColKv + (cc % VP) * DK;
           auto group = [&](int q) { return ta + ((uint32_t)(q / (2 * K::kCg) * 16) << 16) + q % (2 * K::kCg) * 32; };
@@ -1174,12 +1185,10 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             }
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
-              F2 add{r[q & 1][2 * y], r[q & 1][2 * y + 1]};
-              if constexpr (FP16) add = mul2(add, F2{dn[y & 1], dn[y & 1]});
-              float* e = &S[hh][q / 2 % K::kCg][(q & 1) * 16 + 2 * y];
-              const F2 z = fma2(hi, F2{e[0], e[1]}, fma2(lo, F2{e[0], e[1]}, add));
-              e[0] = z.x;
-              e[1] = z.y;
+              F2 add = pack2(r[q & 1][2 * y], r[q & 1][2 * y + 1]);
+              if constexpr (FP16) add = mul2(add, pack2(dn[y & 1], dn[y & 1]));
+              F2& e = S[hh][q / 2 % K::kCg][(q & 1) * 8 + y];
+              e = fma2(hi, e, fma2(lo, e, add));
             }
           }
         }
@@ -1196,13 +1205,17 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
                   if (dv0 + hh * 16 + r * 8 < a.Dv) {
-                    dst[hh * 16 + r * 8] = S[hh][cg][4 * m + 2 * r];
-                    dst[a.Dv + hh * 16 + r * 8] = S[hh][cg][4 * m + 2 * r + 1];
+                    float e, g;
+                    unpack2(S[hh][cg][2 * m + r], e, g);
+                    dst[hh * 16 + r * 8] = e;
+                    dst[a.Dv + hh * 16 + r * 8] = g;
                   }
               }
         }
       }
     }
+
+    if (!ok) give_up(TM && wg == K::kV ? ERR_SITE_DECAY_V : ERR_SITE_DECAY_STATE, w);
   }
 
   tc_fence_before();
