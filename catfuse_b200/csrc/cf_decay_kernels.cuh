@@ -165,6 +165,42 @@ __device__ __forceinline__ void tmem_wait16(float (&r)[16]) {
                  "+r"(u[7]), "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]),
                  "+r"(u[14]), "+r"(u[15])::"memory");
 }
+// 8 N columns of two accumulators (of the first alone if !both), one wait.
+template <int N>
+__device__ __forceinline__ void tmem_ld_pair(uint32_t ta, uint32_t tb, bool both, float (&x)[4 * N], float (&y)[4 * N]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(x);
+  uint32_t* v = reinterpret_cast<uint32_t*>(y);
+  if constexpr (N == 4) {
+    tmem_ld_frag4(ta, x);
+    if (both) tmem_ld_frag4(tb, y);
+    tmem_wait16(x);
+    tmem_wait16(y);
+  } else {
+#define CF_LD8(R, A)                                                                                              \
+  asm volatile(                                                                                                   \
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "                                                                   \
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"                                                   \
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                                  \
+      : "=r"(R[0]), "=r"(R[1]), "=r"(R[2]), "=r"(R[3]), "=r"(R[4]), "=r"(R[5]), "=r"(R[6]), "=r"(R[7]),           \
+        "=r"(R[8]), "=r"(R[9]), "=r"(R[10]), "=r"(R[11]), "=r"(R[12]), "=r"(R[13]), "=r"(R[14]), "=r"(R[15]),     \
+        "=r"(R[16]), "=r"(R[17]), "=r"(R[18]), "=r"(R[19]), "=r"(R[20]), "=r"(R[21]), "=r"(R[22]), "=r"(R[23]),   \
+        "=r"(R[24]), "=r"(R[25]), "=r"(R[26]), "=r"(R[27]), "=r"(R[28]), "=r"(R[29]), "=r"(R[30]), "=r"(R[31])    \
+      : "r"(A)                                                                                                    \
+      : "memory")
+#define CF_WAIT16(R, O, S)                                                                                        \
+  asm volatile(S : "+r"(R[O]), "+r"(R[O + 1]), "+r"(R[O + 2]), "+r"(R[O + 3]), "+r"(R[O + 4]), "+r"(R[O + 5]),    \
+                   "+r"(R[O + 6]), "+r"(R[O + 7]), "+r"(R[O + 8]), "+r"(R[O + 9]), "+r"(R[O + 10]),               \
+                   "+r"(R[O + 11]), "+r"(R[O + 12]), "+r"(R[O + 13]), "+r"(R[O + 14]), "+r"(R[O + 15])::"memory")
+    CF_LD8(u, ta);
+    if (both) CF_LD8(v, tb);
+    CF_WAIT16(u, 0, "tcgen05.wait::ld.sync.aligned;");
+    CF_WAIT16(u, 16, "");
+    CF_WAIT16(v, 0, "");
+    CF_WAIT16(v, 16, "");
+#undef CF_LD8
+#undef CF_WAIT16
+  }
+}
 // 16 rows x 32 words of a packed 16-bit operand: thread t holds row t / 4, word
 // t % 4 of every four, then row t / 4 + 8 (the fragment above, packed in pairs).
 __device__ __forceinline__ void tmem_st_frag8(uint32_t taddr, const uint32_t (&u)[16]) {
@@ -782,13 +818,14 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         Unit x;
         if (!get_unit<OUT>(a, u, x) || x.len == 0) continue;
         const float l2 = log2_decay(a.log_decay[x.h]);
-        F2 f[8][2];  // l^{i-j}, 0 above the diagonal
+        F2 f[8][2];  // scale l^{i-j}, 0 above the diagonal
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int d = i + 8 * r - 8 * n - fc;
-            f[n][r] = pack2(d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1)));
+            f[n][r] = pack2(d < 0 ? 0.f : a.scale * exp2_fast(l2 * (float)d),
+                            d < 1 ? 0.f : a.scale * exp2_fast(l2 * (float)(d - 1)));
           }
         const int items = (x.len + kC - 1) / kC * G;
         for (int k = 0; k < items; ++k, ++it) {
@@ -872,53 +909,57 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           for (int g = 0; g < G; ++g, ++it) {
             if (!(ok = warp_wait(o_full, it & 1, w))) break;
             tc_fence_after();
-            // groups of 16 channels x 32 tokens, one load ahead
-            float p[2][16], z[2][16];
-            tmem_ld_frag4(tlane + K::kColOp, p[0]);
-            tmem_ld_frag4(tlane + K::kColOs, z[0]);
+            // 16 channels x 64 tokens at a time; 32 tokens where registers are few
+            constexpr int NO = K::kCtas == 2 ? 4 : 8;
+            auto put = [&](int hh, auto half) {
+              constexpr int n0 = decltype(half)::value * NO;
+              float p[4 * NO], z[4 * NO];
+              const uint32_t ta = tlane + ((uint32_t)(hh * 16) << 16) + n0 * 8;
+              tmem_ld_pair<NO>(ta + K::kColOp, ta + K::kColOs, has_s, p, z);
+              const bool last = hh == NH - 1 && n0 + NO == 8;
+              if (!FP16 && last) {
+                tc_fence_before();
+                warp_arrive(o_empty);
+              }
+              F2 ss[2];
+              if constexpr (FP16) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const float e = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr + 8 * r];
+                  ss[r] = pack2(e, e);
+                }
+              }
+              uint32_t o[NO][2];
+#pragma unroll
+              for (int n = 0; n < NO; ++n) {
+                F2 pf = 0;
+                if constexpr (FP16) pf = *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + 8 * (n0 + n) + fc]);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  F2 y = pack2(p[4 * n + 2 * r], p[4 * n + 2 * r + 1]);
+                  if constexpr (FP16) y = mul2(y, pf);
+                  if (has_s) {
+                    F2 x2 = pack2(z[4 * n + 2 * r], z[4 * n + 2 * r + 1]);
+                    if constexpr (FP16) x2 = mul2(x2, ss[r]);
+                    y = fma2(grow[n0 + n], x2, y);
+                  }
+                  o[n][r] = Half2<T>::pack(y);
+                }
+              }
+              if (FP16 && last) {  // accumulators and scales are read
+                tc_fence_before();
+                warp_arrive(o_empty);
+              }
+              // block m = lane / 8: tokens 8 (n + m / 2).., channels 8 (m % 2)..
+#pragma unroll
+              for (int n = 0; n < NO; n += 2)
+                stm4_t(stage_u + out_at<kRow>(8 * (n0 + n + (lane >> 4)) + (lane & 7), hh * 2 + ((lane >> 3) & 1)),
+                       o[n][0], o[n][1], o[n + 1][0], o[n + 1][1]);
+            };
 #pragma unroll 1
             for (int hh = 0; hh < NH; ++hh) {
-              float ss[2] = {1.f, 1.f};
-              if constexpr (FP16) {
-                ss[0] = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr];
-                ss[1] = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr + 8];
-              }
-#pragma unroll
-              for (int cg = 0; cg < 2; ++cg) {
-                tmem_wait16(p[cg]);
-                tmem_wait16(z[cg]);
-                if (cg == 0 || hh + 1 < NH) {
-                  const uint32_t ta = tlane + ((uint32_t)((hh + cg) * 16) << 16) + (cg == 0 ? 32 : 0);
-                  tmem_ld_frag4(ta + K::kColOp, p[cg ^ 1]);
-                  tmem_ld_frag4(ta + K::kColOs, z[cg ^ 1]);
-                }
-                uint32_t o[4][2];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                  F2 pf = pack2(a.scale, a.scale);
-                  if constexpr (FP16)
-                    pf = mul2(pf, *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + cg * 32 + 8 * n + fc]));
-#pragma unroll
-                  for (int r = 0; r < 2; ++r) {
-                    F2 y = mul2(pack2(p[cg][4 * n + 2 * r], p[cg][4 * n + 2 * r + 1]), pf);
-                    F2 x2 = pack2(z[cg][4 * n + 2 * r], z[cg][4 * n + 2 * r + 1]);
-                    if constexpr (FP16) x2 = mul2(x2, pack2(ss[r], ss[r]));
-                    if (has_s) y = fma2(grow[cg * 4 + n], x2, y);
-                    o[n][r] = Half2<T>::pack(y);
-                  }
-                }
-                if (hh == NH - 1 && cg == 1) {  // accumulators and scales are read
-                  tc_fence_before();
-                  warp_arrive(o_empty);
-                }
-                // block m = lane / 8: tokens 8 (n + m / 2).., channels 8 (m % 2)..
-#pragma unroll
-                for (int n = 0; n < 4; n += 2) {
-                  const int row = cg * 32 + 8 * (n + (lane >> 4)) + (lane & 7);
-                  stm4_t(stage_u + out_at<kRow>(row, hh * 2 + ((lane >> 3) & 1)), o[n][0], o[n][1], o[n + 1][0],
-                         o[n + 1][1]);
-                }
-              }
+              put(hh, std::integral_constant<int, 0>{});
+              if constexpr (NO == 4) put(hh, std::integral_constant<int, 1>{});
             }
             if (s_badany[cc & 3] == cc + 1)
               spoil_outputs<kRow>(stage, s_bad + (cc & 3) * DV + wq * (DV / 4), cc);
@@ -930,11 +971,13 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
               dst += (int64_t)row0 * a.o_st + v * 8;
               const int64_t step = (int64_t)kRows * a.o_st;
               const int left = dv < a.Dv ? n_tok - row0 : 0;
+              uint4 val[kC / kRows];
+#pragma unroll
+              for (int z = 0; z < kC / kRows; ++z)
+                val[z] = *reinterpret_cast<const uint4*>(stage + out_at<kRow>(z * kRows + row0, v));
 #pragma unroll
               for (int z = 0; z < kC / kRows; ++z, dst += step)
-                if (z * kRows < left)
-                  *reinterpret_cast<uint4*>(dst) =
-                      *reinterpret_cast<const uint4*>(stage + out_at<kRow>(z * kRows + row0, v));
+                if (z * kRows < left) *reinterpret_cast<uint4*>(dst) = val[z];
             } else {
               store_unaligned<T, kRow>(stage, dst, a.o_st, n_tok, a.Dv - wq * (DV / 4));
             }
@@ -1011,9 +1054,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             if ((lane & 3) == 0) s_vscale[(chunk & 3) * 128 + d0 + fr + 8 * r] = pow2i(-e);
           }
         }
-        uint32_t part[K::kVParts][16];
-#pragma unroll
-        for (int h = 0; h < 16; h += 8) {
+        auto split8 = [&](int h, uint32_t (*part)[16], int o) {
           F2 g[8];
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
@@ -1024,24 +1065,34 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           for (int p = 0; p < K::kVParts; ++p)
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
-              part[p][h + y] = Half2<T>::pack(g[y]);
-              if (p + 1 < K::kVParts) g[y] = sub2(g[y], Half2<T>::unpack(part[p][h + y]));
+              part[p][o + y] = Half2<T>::pack(g[y]);
+              if (p + 1 < K::kVParts) g[y] = sub2(g[y], Half2<T>::unpack(part[p][o + y]));
             }
+        };
+        uint32_t part[K::kVParts][16];
+        if constexpr (TM) {
+          split8(0, part, 0);
+          split8(8, part, 8);
         }
         // KV of the chunk before in this buffer has read its V'
         if (hh == 0) {
           if (!warp_wait(&ds_full[chunk % VP], ((chunk / VP) & 1) ^ 1, w)) return false;
           tc_fence_after();
         }
+        if constexpr (TM) {
 #pragma unroll
-        for (int q = 0; q < K::kVParts; ++q) {
-          if constexpr (TM) {
+          for (int q = 0; q < K::kVParts; ++q)
             tmem_st_frag8(tlane + ((uint32_t)(hh * 16) << 16) + K::kColV + ((chunk % VP) * K::kVParts + q) * 32, part[q]);
-          } else {
-            const uint32_t to = smem_u32(sVp) + q * K::kVBytes + (at - vu);
+        } else {
 #pragma unroll
-            for (int z = 0; z < 4; ++z)
-              stm4_t(to + z * 2048, part[q][4 * z], part[q][4 * z + 1], part[q][4 * z + 2], part[q][4 * z + 3]);
+          for (int h = 0; h < 16; h += 8) {
+            split8(h, part, 0);
+#pragma unroll
+            for (int q = 0; q < K::kVParts; ++q) {
+              const uint32_t to = smem_u32(sVp) + q * K::kVBytes + (at - vu) + h * 512;
+              stm4_t(to, part[q][0], part[q][1], part[q][2], part[q][3]);
+              stm4_t(to + 2048, part[q][4], part[q][5], part[q][6], part[q][7]);
+            }
           }
         }
       }
@@ -1080,23 +1131,51 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         const float ld = a.log_decay[x.h], l2 = log2_decay(ld);
         const float2 whole = pow_hi_lo(ld, kC), tail = pow_hi_lo(ld, x.len & (kC - 1));
         const int64_t at = (int64_t)fc * a.Dv + dv0;
+        if (x.start && a.Dk == DK && a.Dv == DV) {  // all loads in flight at once
+          const float* src = x.start + fc * DV + dv0;
+          float e[NH][K::kCg][32];
 #pragma unroll
-        for (int hh = 0; hh < NH; ++hh)
+          for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
-          for (int cg = 0; cg < K::kCg; ++cg)
+            for (int cg = 0; cg < K::kCg; ++cg)
 #pragma unroll
-            for (int m = 0; m < 8; ++m) {
-              const bool in = x.start && cg * 64 + m * 8 < a.Dk;
-              const float* src = x.start + at + (cg * 64 + m * 8) * a.Dv;
+              for (int y = 0; y < 32; ++y)
+                e[hh][cg][y] = src[(cg * 64 + (y >> 2) * 8 + (y & 1)) * DV + hh * 16 + (y >> 1 & 1) * 8];
 #pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const bool on = in && dv0 + hh * 16 + r * 8 < a.Dv;
-                S[hh][cg][2 * m + r] = on ? pack2(src[hh * 16 + r * 8], src[a.Dv + hh * 16 + r * 8]) : 0;
-              }
-            }
+          for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+            for (int cg = 0; cg < K::kCg; ++cg)
+#pragma unroll
+              for (int y = 0; y < 16; ++y) S[hh][cg][y] = pack2(e[hh][cg][2 * y], e[hh][cg][2 * y + 1]);
+        } else {
+#pragma unroll
+          for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+            for (int cg = 0; cg < K::kCg; ++cg)
+#pragma unroll
+              for (int y = 0; y < 16; ++y) S[hh][cg][y] = 0;
+          if (x.start) {
+#pragma unroll
+            for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+              for (int cg = 0; cg < K::kCg; ++cg)
+#pragma unroll
+                for (int y = 0; y < 16; ++y) {
+                  const int dk = cg * 64 + (y >> 1) * 8, dv = hh * 16 + (y & 1) * 8;
+                  if (dk < a.Dk && dv0 + dv < a.Dv) {
+                    const float* src = x.start + at + dk * a.Dv + dv;
+                    S[hh][cg][y] = pack2(src[0], src[a.Dv]);
+                  }
+                }
+          }
+        }
         F2 f[8];
         for (int c = 0; c < x.len; c += kC, ++cc) {
           const int n = min(kC, x.len - c);
+          if constexpr (!TM) {  // before S, so that KV runs while S is put
+            if (c == 0 || n < kC) factors(l2, n, f);
+            if (!(ok = put_v(cc, n, f))) break;
+          }
           if (OUT && (c > 0 || x.start)) {
             // S^T in 16 bits, for the product with the queries; the one before it
             // is done when s_empty comes round
@@ -1154,10 +1233,6 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             }
             warp_arrive(s_full);
             ++ns;
-          }
-          if constexpr (!TM) {
-            if (c == 0 || n < kC) factors(l2, n, f);
-            if (!(ok = put_v(cc, n, f))) break;
           }
           if (!(ok = warp_wait(&ds_full[cc % VP], (cc / VP) & 1, w))) break;
           tc_fence_after();
