@@ -9,7 +9,7 @@
 // that enter the segments, and the walk then runs per segment.
 #include "cf_decay_kernels.cuh"
 
-#include <atomic>
+#include <cmath>
 #include <mutex>
 
 namespace cf {
@@ -232,15 +232,13 @@ struct Plan {
 };
 
 // How long the segments are.  Times in units of one chunk of a single query
-// head: the walk takes 1 for a chunk and its first query head and about 0.4 for
-// every further one, the pass that sums states 0.5, and the three launches of a
-// cut call cost about 8 more than the one of an uncut call.
+// head: the walk takes 1 for a chunk and its first query head and about 0.7 for
+// every further one, the pass that sums states 0.6; a segment costs 3 on top (its
+// state comes and goes, its pipeline fills), a cut call's two more launches 8.
 Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t Dv, bool packed, int sms) {
   Plan p{};
-  const int64_t ctas = sms * ((Dk <= 64 && Dv <= 64) ? 2 : 1);
+  const double t_walk = 1.0 + 0.7 * ((double)Hq / Hk - 1.0), t_sum = 0.6, t_cut = 8.0, t_unit = 3.0;
   const int64_t units = S * Hk;
-  const double t_walk = 1.0 + 0.4 * ((double)Hq / Hk - 1.0), t_sum = 0.5, t_cut = 8.0,
-               t_unit = 3.0;
   p.n_segs = S;
   p.n_seg = 1;
   p.seg_len = N > kC ? (N + kC - 1) / kC * kC : kC;
@@ -248,10 +246,10 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
     if (!packed) {
       const int64_t ch = (N / S + kC - 1) / kC;
       double best = 0;
-      for (int64_t n = 1; n <= ch && n <= 1024; ++n) {
+      for (int64_t n = 1; n <= ch && n <= 256; ++n) {
         const int64_t len = (ch + n - 1) / n;
         if ((ch + len - 1) / len != n) continue;
-        const double waves = (double)((units * n + ctas - 1) / ctas);
+        const double waves = (double)((units * n + sms - 1) / sms);
         const double waves_s = (double)((units * (n - 1) + sms - 1) / sms);
         const double t = waves * (len * t_walk + t_unit) + (n > 1 ? waves_s * (len * t_sum + t_unit) + t_cut : 0.0);
         if (n == 1 || t < best) {
@@ -263,10 +261,12 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
       p.n_segs = S * p.n_seg;
       p.split = p.n_seg > 1;
     } else {
-      // Lengths are on the device: segments of an equal share of all chunks, so
-      // that one long sequence among short ones does not run alone at the end.
-      const int64_t share = (N / kC * Hk + ctas - 1) / ctas;
-      const int64_t len = share > 16 ? share : 16;
+      // Lengths are on the device.  The shorter the segments, the more evenly
+      // they spread (half a segment is lost at the end), and the more of them
+      // there are to set up: of c chunks for each CTA, c / len segments.
+      const double c = (double)(N / kC + S) * Hk / sms;
+      int64_t len = (int64_t)sqrt(2.0 * c * t_unit / t_walk) + 1;
+      if (len < 4) len = 4;
       if (N > len * kC) {
         p.seg_len = len * kC;
         p.n_segs = S + N / p.seg_len;

@@ -11,8 +11,19 @@
 //
 // The angle is reduced in fp64 (turns = pos * inv_freq / 2 pi, minus the nearest
 // whole number): in fp32 the product alone is 2e-3 radians off at position
-// 32768, more than bf16 rounds away.  One sine and cosine per (token, pair) is
-// put into shared memory and serves all heads of the token.
+// 32768, more than bf16 rounds away.
+//
+// A warp owns a token (or a share of its heads where tokens are few): each lane
+// takes the sine and cosine of a few pairs and the warp exchanges them once.  Every
+// lane then keeps, for its own channels, sines and cosines times the norm's weights
+// in registers for all heads of the token:
+//
+//   a' = inv (a (wa cos) - b (wb sin)),   b' = inv (b (wb cos) + a (wa sin))
+//
+// so a head costs one load, one sum over the row's lanes, two products of two values
+// at a time per pair, and one store, with the next two rows' loads in flight.
+// (With weights and rotation applied one after the other and a rounded square root
+// and division, it was bound by instructions: 390 for four rows of 128 channels.)
 #include "cf_half.cuh"
 
 namespace cf {
@@ -21,8 +32,6 @@ namespace {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxDim = 256;
 constexpr int kRopeMaxAxes = 4;
-constexpr int kRopeMaxTokens = 16;      // tokens of one CTA
-constexpr int kRopeTableBytes = 16 << 10;  // cosines and sines of one CTA
 
 struct RopeArgs {
   const void* q;
@@ -37,7 +46,8 @@ struct RopeArgs {
   const float* q_weight;
   const float* k_weight;
   int64_t N;
-  int Hq, Hk, D, rot, half_pairs, norm, tok;  // half_pairs: pairs are (p, p + rot/2)
+  int Hq, Hk, D, rot, half_pairs, norm;  // half_pairs: pairs are (p, p + rot/2)
+  int lpr, splits;  // lanes of a row, warps of a token
   float eps;
   uint8_t axis[kRopeMaxDim / 2];
 };
@@ -54,14 +64,13 @@ template <typename T>
 struct RopeVec<T, 1> { using type = uint16_t; };
 
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&f)[V]) {
-  typename RopeVec<T, V>::type raw = *reinterpret_cast<const typename RopeVec<T, V>::type*>(p);
+__device__ __forceinline__ void to_floats(const typename RopeVec<T, V>::type& raw, float* f) {
   const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = to_f(e[i]);
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
+__device__ __forceinline__ void store_vec(T* p, const float* f) {
   typename RopeVec<T, V>::type raw;
   T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
@@ -69,127 +78,234 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
   *reinterpret_cast<typename RopeVec<T, V>::type*>(p) = raw;
 }
 
-__device__ __forceinline__ void turn(float& a, float& b, float2 cs) {
-  const float u = a, v = b;
-  a = u * cs.x - v * cs.y;
-  b = v * cs.x + u * cs.y;
+// Two fp32 values at a time, in a register pair.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 pack2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(F2 a, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a));
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 // A lane owns U units of a row, a unit being two vectors of V channels that
-// hold V whole pairs (or 2V channels that pass through); lpr <= 32 lanes own a row.
+// hold V whole pairs (or 2V channels that pass through); lpr lanes own a row.
 template <typename T, int V, int U>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a,
-                                                                   int lpr) {
-  extern __shared__ float2 s_cs[];  // [tokens of this CTA][rot / 2]
-  const int P = a.rot / 2;
-  const int64_t t0 = (int64_t)blockIdx.x * a.tok;
-  const int nt = a.N - t0 < a.tok ? (int)(a.N - t0) : a.tok;
-  for (int i = threadIdx.x; i < nt * P; i += kRopeThreads) {
-    const int t = i / P, p = i - t * P;
-    const int64_t at = a.axis[p] * a.pos_stride + t0 + t;
+__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+  __shared__ float2 s_cs[kRopeThreads / 32][kRopeMaxDim / 2];
+  __shared__ __align__(16) float s_w[2][kRopeMaxDim];
+  using Vec = typename RopeVec<T, V>::type;
+  const int lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
+  const int64_t t = min(id / a.splits, a.N - 1);
+  const int split = (int)(id - id / a.splits * a.splits);
+  const int P = a.rot / 2, RU = a.rot / (2 * V), NU = a.D / (2 * V);
+  const int lpr = a.lpr, sub = lane & (lpr - 1), rows = 32 / lpr;
+  const int itq = (a.Hq + rows - 1) / rows, its = itq + (a.Hk + rows - 1) / rows;
+  const int first = its * split / a.splits, end = id / a.splits < a.N ? its * (split + 1) / a.splits : 0;
+  int ca[U], cb[U];  // first channels of the two vectors
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    const int unit = sub + j * lpr;
+    const bool apart = a.half_pairs && unit < RU;
+    ca[j] = apart ? unit * V : 2 * unit * V;
+    cb[j] = apart ? ca[j] + P : ca[j] + V;
+  }
+  const T* const q = static_cast<const T*>(a.q) + t * a.q_st;
+  const T* const k = static_cast<const T*>(a.k) + t * a.k_st;
+  T* const qo = static_cast<T*>(a.q_out) + t * a.qo_st;
+  T* const ko = static_cast<T*>(a.k_out) + t * a.ko_st;
+  // rows it * rows .. of the queries, then of the keys
+  auto head = [&](int it) { return (it < itq ? it : it - itq) * rows + lane / lpr; };
+  auto on = [&](int it) { return it < end && head(it) < (it < itq ? a.Hq : a.Hk); };
+  auto load = [&](int it, Vec (&x)[U], Vec (&y)[U]) {
+    const T* src = it < itq ? q + head(it) * a.q_sh : k + head(it) * a.k_sh;
+    const bool in = on(it);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      x[j] = y[j] = Vec{};
+      if (in && sub + j * lpr < NU) {
+        x[j] = *reinterpret_cast<const Vec*>(src + ca[j]);
+        y[j] = *reinterpret_cast<const Vec*>(src + cb[j]);
+      }
+    }
+  };
+  constexpr int B = 2;  // rows of a batch; the next batch is loaded while one is worked on
+  Vec nx[B][U], ny[B][U];
+#pragma unroll
+  for (int b = 0; b < B; ++b) load(first + b, nx[b], ny[b]);
+
+  for (int i = threadIdx.x; i < 2 * a.D; i += kRopeThreads) {
+    const float* w = a.norm ? (i < a.D ? a.q_weight : a.k_weight) : nullptr;
+    const int c = i < a.D ? i : i - a.D;
+    s_w[i >= a.D][c] = w ? w[c] : 1.f;
+  }
+  float2* cs = s_cs[threadIdx.x >> 5];
+  for (int p = lane; p < P; p += 32) {
+    const int64_t at = a.axis[p] * a.pos_stride + t;
     const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at]
                                : (double)static_cast<const int32_t*>(a.pos)[at];
     const double turns = pos * (double)a.inv_freq[p] * 0.15915494309189533577;
     float s, c;
     sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    s_cs[i] = make_float2(c, s);
+    cs[p] = make_float2(c, s);
   }
   __syncthreads();
 
-  const int H = a.Hq + a.Hk;
-  const int lane = threadIdx.x & (lpr - 1);
-  const int rows_at_once = kRopeThreads / lpr;
-  const int RU = a.rot / (2 * V), NU = a.D / (2 * V);
-  // every lane of a warp takes part in the row sums, also beyond the last row
-  const int n_rows = nt * H;
-  for (int r0 = 0; r0 < n_rows; r0 += rows_at_once) {
-    const int r = r0 + threadIdx.x / lpr;
-    const bool on = r < n_rows;
-    const int t = on ? r / H : 0;
-    const int h = on ? r - t * H : 0;
-    const bool is_q = h < a.Hq;
-    const int hh = is_q ? h : h - a.Hq;
-    const T* src = is_q ? static_cast<const T*>(a.q) + (t0 + t) * a.q_st + hh * a.q_sh
-                        : static_cast<const T*>(a.k) + (t0 + t) * a.k_st + hh * a.k_sh;
-    T* dst = is_q ? static_cast<T*>(a.q_out) + (t0 + t) * a.qo_st + hh * a.qo_sh
-                  : static_cast<T*>(a.k_out) + (t0 + t) * a.ko_st + hh * a.ko_sh;
-    float x[U][V], y[U][V];
-    int ca[U], cb[U];  // first channels of the two vectors
+  // Coefficients of x and y, the lane's two vectors, two values at a time:
+  // pairs across the vectors: x' = x c0 + y c1, y' = y c2 + x c3;
+  // pairs within a vector:    x' = x c0 + swap(x) c1, y' = y c2 + swap(y) c3.
+  // One value in place of two where V = 1 (the second is unused).
+  constexpr int H = V > 1 ? V / 2 : 1;
+  F2 c0[U][H], c1[U][H], c2[U][H], c3[U][H];
+  auto coefficients = [&](const float* wt) {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int unit = lane + j * 32;
-      const bool split = a.half_pairs && unit < RU;
-      ca[j] = split ? unit * V : 2 * unit * V;
-      cb[j] = split ? ca[j] + P : ca[j] + V;
+      const int unit = sub + j * lpr;
+      const bool in = unit < NU, turned = unit < RU;
+      float wa[2 * H], wb[2 * H], c[2 * H], s[2 * H];
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[j][i] = y[j][i] = 0.f;
-      if (on && unit < NU) {
-        load_vec<T, V>(src + ca[j], x[j]);
-        load_vec<T, V>(src + cb[j], y[j]);
+      for (int i = 0; i < V; ++i) {
+        wa[i] = in ? wt[ca[j] + i] : 0.f;
+        wb[i] = in ? wt[cb[j] + i] : 0.f;
+        const float2 z = turned ? cs[unit * V + i] : make_float2(1.f, 0.f);
+        c[i] = z.x;
+        s[i] = z.y;
+      }
+      if (V == 1) wa[1] = wb[1] = c[1] = s[1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const int e = 2 * i, f = 2 * i + 1;
+        if (a.half_pairs || V == 1) {
+          c0[j][i] = pack2(wa[e] * c[e], wa[f] * c[f]);
+          c1[j][i] = pack2(-wb[e] * s[e], -wb[f] * s[f]);
+          c2[j][i] = pack2(wb[e] * c[e], wb[f] * c[f]);
+          c3[j][i] = pack2(wa[e] * s[e], wa[f] * s[f]);
+        } else {  // vector x holds pairs 0 .. V/2 - 1, y the others
+          const float cx = c[i], sx = s[i], cy = c[V / 2 + i], sy = s[V / 2 + i];
+          c0[j][i] = pack2(wa[e] * cx, wa[f] * cx);
+          c1[j][i] = pack2(-wa[f] * sx, wa[e] * sx);
+          c2[j][i] = pack2(wb[e] * cy, wb[f] * cy);
+          c3[j][i] = pack2(-wb[f] * sy, wb[e] * sy);
+        }
       }
     }
-    if (a.norm) {
-      float ss = 0.f;
+  };
+  const float inv_d = 1.f / (float)a.D;
+  bool keys = first >= itq;
+  coefficients(s_w[keys]);
+  for (int it = first; it < end; it += B) {
+    Vec rx[B][U], ry[B][U];
 #pragma unroll
-      for (int j = 0; j < U; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) ss += x[j][i] * x[j][i] + y[j][i] * y[j][i];
-      for (int m = lpr >> 1; m; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-      const float inv = 1.f / sqrtf(ss / (float)a.D + a.eps);
-      const float* w = is_q ? a.q_weight : a.k_weight;
+    for (int b = 0; b < B; ++b)
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        if (lane + j * 32 >= NU) continue;
+        rx[b][j] = nx[b][j];
+        ry[b][j] = ny[b][j];
+      }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[j][i] *= w ? inv * __ldg(w + ca[j] + i) : inv;
-          y[j][i] *= w ? inv * __ldg(w + cb[j] + i) : inv;
+    for (int b = 0; b < B; ++b) load(it + B + b, nx[b], ny[b]);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      if (it + b >= end) break;
+      if (!keys && it + b >= itq) {
+        keys = true;
+        coefficients(s_w[1]);
+      }
+      F2 x[U][H], y[U][H];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        float e[2 * H], f[2 * H];
+        e[2 * H - 1] = f[2 * H - 1] = 0.f;
+        to_floats<T, V>(rx[b][j], e);
+        to_floats<T, V>(ry[b][j], f);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          x[j][i] = pack2(e[2 * i], e[2 * i + 1]);
+          y[j][i] = pack2(f[2 * i], f[2 * i + 1]);
         }
       }
-    }
-    if (!on) continue;
+      float inv = 1.f;
+      if (a.norm) {
+        F2 sum = 0;
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int unit = lane + j * 32;
-      if (unit >= NU) continue;
-      if (unit < RU) {
-        const float2* cs = s_cs + t * P + unit * V;
-        if (a.half_pairs || V == 1) {
+        for (int j = 0; j < U; ++j)
 #pragma unroll
-          for (int i = 0; i < V; ++i) turn(x[j][i], y[j][i], cs[i]);
-        } else {
+          for (int i = 0; i < H; ++i) sum = fma2(x[j][i], x[j][i], fma2(y[j][i], y[j][i], sum));
+        float ss, s1;
+        unpack2(sum, ss, s1);
+        ss += s1;
+        for (int m = lpr >> 1; m; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+        inv = rsqrtf(fmaf(ss, inv_d, a.eps));
+      }
+      const F2 inv2 = pack2(inv, inv);
+      const bool put = on(it + b);
+      T* dst = it + b < itq ? qo + head(it + b) * a.qo_sh : ko + head(it + b) * a.ko_sh;
 #pragma unroll
-          for (int i = 0; i + 1 < V; i += 2) {
-            turn(x[j][i], x[j][i + 1], cs[i / 2]);
-            turn(y[j][i], y[j][i + 1], cs[V / 2 + i / 2]);
+      for (int j = 0; j < U; ++j) {
+        float e[2 * H], f[2 * H];
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          F2 p = x[j][i], r = y[j][i];  // what meets c1 and c3
+          if (a.half_pairs || V == 1) {
+            p = y[j][i];
+            r = x[j][i];
+          } else {
+            float u, v;
+            unpack2(p, u, v);
+            p = pack2(v, u);
+            unpack2(r, u, v);
+            r = pack2(v, u);
           }
+          unpack2(mul2(fma2(p, c1[j][i], mul2(x[j][i], c0[j][i])), inv2), e[2 * i], e[2 * i + 1]);
+          unpack2(mul2(fma2(r, c3[j][i], mul2(y[j][i], c2[j][i])), inv2), f[2 * i], f[2 * i + 1]);
+        }
+        if (put && sub + j * lpr < NU) {
+          store_vec<T, V>(dst + ca[j], e);
+          store_vec<T, V>(dst + cb[j], f);
         }
       }
-      store_vec<T, V>(dst + ca[j], x[j]);
-      store_vec<T, V>(dst + cb[j], y[j]);
     }
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, int U>
 int launch_rope(const RopeArgs& a, cudaStream_t s) {
-  constexpr int U = kRopeMaxDim / (2 * V) > 32 ? kRopeMaxDim / (2 * V) / 32 : 1;
-  int lpr = 1;
-  while (lpr < 32 && lpr < a.D / (2 * V)) lpr <<= 1;
-  const int64_t grid = (a.N + a.tok - 1) / a.tok;
-  qk_norm_rope_kernel<T, V, U>
-      <<<(unsigned)grid, kRopeThreads, (size_t)a.tok * (a.rot / 2) * 8, s>>>(a, lpr);
+  constexpr int kWarps = kRopeThreads / 32;
+  const int64_t grid = (a.N * a.splits + kWarps - 1) / kWarps;
+  qk_norm_rope_kernel<T, V, U><<<(unsigned)grid, kRopeThreads, 0, s>>>(a);
   return check_launch("qk_norm_rope launch");
 }
 
+// As few lanes a row as keep U V <= 8: more rows a warp, and more loads in
+// flight a lane (80 channels in 4-byte vectors: 8 lanes x 3 units instead of 32 x 1).
 template <typename T>
-int launch_rope_v(const RopeArgs& a, int V, cudaStream_t s) {
-  switch (V) {
-    case 8: return launch_rope<T, 8>(a, s);
-    case 4: return launch_rope<T, 4>(a, s);
-    case 2: return launch_rope<T, 2>(a, s);
-    default: return launch_rope<T, 1>(a, s);
-  }
+int launch_rope_v(RopeArgs a, int V, cudaStream_t s) {
+  const int units = a.D / (2 * V);
+  a.lpr = 1;
+  while (a.lpr < 32 && a.lpr * (8 / V) < units) a.lpr <<= 1;
+  const int U = (units + a.lpr - 1) / a.lpr, rows = 32 / a.lpr;
+  // Tokens that do not fill the GPU share their heads out over more warps.
+  const int its = (a.Hq + rows - 1) / rows + (a.Hk + rows - 1) / rows;
+  const int64_t want = (148 * 16 + a.N - 1) / a.N;
+  a.splits = (int)(want < its ? want : its);
+  if (V == 8) return launch_rope<T, 8, 1>(a, s);
+  if (V == 4) return U == 1 ? launch_rope<T, 4, 1>(a, s) : launch_rope<T, 4, 2>(a, s);
+  if (V == 2)
+    return U == 1 ? launch_rope<T, 2, 1>(a, s) : U == 2 ? launch_rope<T, 2, 2>(a, s)
+         : U == 3 ? launch_rope<T, 2, 3>(a, s) : launch_rope<T, 2, 4>(a, s);
+  return launch_rope<T, 1, 8>(a, s);
 }
 
 }  // namespace
@@ -268,9 +384,7 @@ extern "C" int cf_qk_norm_rope(const void* q, const void* k, void* q_out, void* 
   a.inv_freq = inv_freq; a.q_weight = q_weight; a.k_weight = k_weight;
   a.N = N; a.Hq = (int)Hq; a.Hk = (int)Hk; a.D = (int)D; a.rot = (int)rot;
   a.half_pairs = pairing == CF_PAIR_HALF; a.norm = norm; a.eps = eps;
-  a.tok = 4;
-  if (a.tok * (rot / 2) * 8 > kRopeTableBytes) a.tok = 1;
-  if ((N + a.tok - 1) / a.tok > 0x7FFFFFFF) return fail(CF_ERR_UNSUPPORTED, "too many tokens");
+  if (N > 0x7FFFFFFF) return fail(CF_ERR_UNSUPPORTED, "too many tokens");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return fmt == CF_FMT_F16 ? launch_rope_v<__half>(a, V, s) : launch_rope_v<__nv_bfloat16>(a, V, s);
 }

@@ -7,6 +7,7 @@ a CPU tensor or a missing library raises.
 """
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 from typing import Optional
 
@@ -69,7 +70,8 @@ def pad16(c: int) -> int:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the handle alone: building a torch.cuda.Stream costs 3 us a call
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -635,34 +637,49 @@ def conv_bn_lif_dual(x: torch.Tensor, wp: torch.Tensor, scale: torch.Tensor, shi
 
 _HALF_FORMATS = {torch.float16: FMT_F16, torch.bfloat16: FMT_BF16}
 _PAIRINGS = {"half": PAIR_HALF, "adjacent": PAIR_ADJACENT}
+_POSITION_BITS = {torch.int32: 32, torch.int64: 64}
 _AXIS_ORDERS = {"blocks": AXES_BLOCKS, "cyclic": AXES_CYCLIC}
 
 
-def _on_device(t: torch.Tensor, name: str, dtype=None):
-    """A CUDA tensor of the current device (the launch goes to its stream)."""
+def _current_device(t: torch.Tensor, name: str) -> torch.device:
+    """The device of a CUDA tensor, which must be the current one (the launch
+    goes to its stream)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
+    dev = t.device
+    if dev.type != "cuda":
         raise CatfuseNativeError(f"{name} must be a CUDA tensor (no CPU path exists)",
                                  _lib.CF_ERR_INVALID_ARG)
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, not on the current device")
-    if dtype is not None and t.dtype != dtype:
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {dev}, not on the current device")
+    return dev
+
+
+def _on(dev: torch.device, t: torch.Tensor, name: str, dtype):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device != dev:
+        if t.device.type != "cuda":
+            _current_device(t, name)
+        raise ValueError(f"{name} is on {t.device}, not on {dev}")
+    if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    return t
 
 
 def _head_strides(t: torch.Tensor, name: str):
     """Token and head strides of t[..., H, D]: the leading axes must collapse
     into one token axis and channels must be adjacent."""
-    st, shape = t.stride(), t.shape
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] != 1:
+        raise ValueError(f"the channels of {name} must be adjacent")
+    n = len(st)
+    if n == 3:
+        return st[0], st[1]
+    shape = t.shape
     if not t.numel():
         return 0, 0
-    if shape[-1] != 1 and st[-1] != 1:
-        raise ValueError(f"the channels of {name} must be adjacent")
-    token = 0
-    span = 1
-    for i in range(len(shape) - 3, -1, -1):
+    token, span = 0, 1
+    for i in range(n - 3, -1, -1):
         if shape[i] == 1:
             continue
         if span == 1:
@@ -673,40 +690,51 @@ def _head_strides(t: torch.Tensor, name: str):
     return token, st[-2]
 
 
-def _states(t: torch.Tensor, name: str, shape):
-    _on_device(t, name, torch.float32)
-    if t.dim() != 4 or tuple(t.shape[1:]) != shape:
+def _states(dev, t: torch.Tensor, name: str, shape):
+    _on(dev, t, name, torch.float32)
+    if t.shape[1:] != shape:
         raise ValueError(f"{name} must be [rows, {shape[0]}, {shape[1]}, {shape[2]}] fp32")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.shape[0]
 
 
-def _decay_args(q, k, v, log_decay, out, lead):
-    """Shape checks that prompts and single tokens share -> (fmt, Hq, Hk, Dk, Dv, out)."""
-    _on_device(q, "q")
-    fmt = _HALF_FORMATS.get(q.dtype)
+def _slots(dev, slots, n):
+    if slots is None:
+        return None
+    _on(dev, slots, "slots", torch.int32)
+    if slots.shape != (n,) or not slots.is_contiguous():
+        raise ValueError(f"slots must be a contiguous [{n}] tensor")
+    return slots.data_ptr()
+
+
+def _decay_args(q, k, v, log_decay, out, dims):
+    """Checks that prompts and single tokens share -> (device, format, Hq, Hk, Dk, Dv, out)."""
+    dev = _current_device(q, "q")
+    dtype = q.dtype
+    fmt = _HALF_FORMATS.get(dtype)
     if fmt is None:
-        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
-    _on_device(k, "k", q.dtype)
-    _on_device(v, "v", q.dtype)
-    if q.dim() != lead + 2 or k.dim() != lead + 2 or v.dim() != lead + 2:
-        raise ValueError(f"q, k and v must have {lead + 2} dimensions")
-    if k.shape[:-2] != q.shape[:-2] or v.shape[:-1] != k.shape[:-1] or k.shape[-1] != q.shape[-1]:
+        raise TypeError(f"q must be fp16 or bf16, got {dtype}")
+    for t, n in ((k, "k"), (v, "v")):
+        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dtype:
+            _on(dev, t, n, dtype)
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != dims or len(ks) != dims or len(vs) != dims:
+        raise ValueError(f"q, k and v must have {dims} dimensions")
+    if ks[:-2] != qs[:-2] or vs[:-1] != ks[:-1] or ks[-1] != qs[-1]:
         raise ValueError("q [..., Hq, Dk], k [..., Hk, Dk] and v [..., Hk, Dv] do not match")
-    Hq, Dk = q.shape[-2:]
-    Hk, Dv = v.shape[-2:]
-    _on_device(log_decay, "log_decay", torch.float32)
-    if log_decay.numel() != Hk or not log_decay.is_contiguous():
+    Hk, Dv = vs[-2:]
+    _on(dev, log_decay, "log_decay", torch.float32)
+    if log_decay.shape != (Hk,) or not log_decay.is_contiguous():
         raise ValueError(f"log_decay must hold Hk={Hk} contiguous values")
-    shape = (*q.shape[:-1], Dv)
+    shape = (*qs[:-1], Dv)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     else:
-        _on_device(out, "out", q.dtype)
-        if tuple(out.shape) != shape:
+        _on(dev, out, "out", dtype)
+        if out.shape != shape:
             raise ValueError(f"out must be {list(shape)}")
-    return fmt, Hq, Hk, Dk, Dv, out
+    return dev, fmt, qs[-2], Hk, qs[-1], Dv, out
 
 
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -724,28 +752,25 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     names the row of each sequence (outside the rows: start from zeros, store
     nothing).  Returns out [..., Hq, Dv]."""
     packed = cu_seqlens is not None
-    fmt, Hq, Hk, Dk, Dv, out = _decay_args(q, k, v, log_decay, out, 1 if packed else 2)
+    dev, fmt, Hq, Hk, Dk, Dv, out = _decay_args(q, k, v, log_decay, out, 3 if packed else 4)
     if packed:
-        _on_device(cu_seqlens, "cu_seqlens", torch.int32)
+        _on(dev, cu_seqlens, "cu_seqlens", torch.int32)
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or not cu_seqlens.is_contiguous():
             raise ValueError("cu_seqlens must be a contiguous [S + 1] tensor")
         S, L, N = cu_seqlens.numel() - 1, 0, q.shape[0]
     else:
         S, L = q.shape[:2]
         N = S * L
-    rows = [_states(t, n, (Hk, Dk, Dv)) for t, n in ((s_in, "s_in"), (s_out, "s_out")) if t is not None]
+    rows = [_states(dev, t, n, (Hk, Dk, Dv)) for t, n in ((s_in, "s_in"), (s_out, "s_out")) if t is not None]
     if len(rows) == 2 and rows[0] != rows[1]:
         raise ValueError("s_in and s_out must have the same number of rows")
-    if slots is not None:
-        _on_device(slots, "slots", torch.int32)
-        if tuple(slots.shape) != (S,) or not slots.is_contiguous():
-            raise ValueError(f"slots must be a contiguous [{S}] tensor")
+    slots_ptr = _slots(dev, slots, S)
     need = _lib.load().cf_decay_attention_workspace(S, N, Hq, Hk, Dk, Dv, packed)
     if need < 0:
         _lib.check(need, "cf_decay_attention_workspace")
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.call("cf_decay_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), fmt,
-              log_decay.data_ptr(), _ptr(s_in), _ptr(s_out), _ptr(slots), rows[0] if rows else 0,
+              log_decay.data_ptr(), _ptr(s_in), _ptr(s_out), slots_ptr, rows[0] if rows else 0,
               _ptr(cu_seqlens), S, L, N, Hq, Hk, Dk, Dv, *_head_strides(q, "q"),
               *_head_strides(k, "k"), *_head_strides(v, "v"), *_head_strides(out, "out"),
               float(Dk ** -0.5 if scale is None else scale), _ptr(ws), need, _stream())
@@ -761,19 +786,15 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     [rows, Hk, Dk, Dv] are updated in place, or written to ``s_out``; ``slots``
     int32 [B] names the row of each sequence (outside the rows: a padding entry,
     zero output, no state touched)."""
-    fmt, Hq, Hk, Dk, Dv, out = _decay_args(q, k, v, log_decay, out, 1)
+    dev, fmt, Hq, Hk, Dk, Dv, out = _decay_args(q, k, v, log_decay, out, 3)
     B = q.shape[0]
-    rows = _states(s_in, "s_in", (Hk, Dk, Dv))
+    rows = _states(dev, s_in, "s_in", (Hk, Dk, Dv))
     if s_out is None:
         s_out = s_in
-    elif _states(s_out, "s_out", (Hk, Dk, Dv)) != rows:
+    elif _states(dev, s_out, "s_out", (Hk, Dk, Dv)) != rows:
         raise ValueError("s_in and s_out must have the same number of rows")
-    if slots is not None:
-        _on_device(slots, "slots", torch.int32)
-        if tuple(slots.shape) != (B,) or not slots.is_contiguous():
-            raise ValueError(f"slots must be a contiguous [{B}] tensor")
     _lib.call("cf_decay_attention_step", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-              fmt, log_decay.data_ptr(), s_in.data_ptr(), s_out.data_ptr(), _ptr(slots), rows, B,
+              fmt, log_decay.data_ptr(), s_in.data_ptr(), s_out.data_ptr(), _slots(dev, slots, B), rows, B,
               Hq, Hk, Dk, Dv, *_head_strides(q, "q"), *_head_strides(k, "k"),
               *_head_strides(v, "v"), *_head_strides(out, "out"),
               float(Dk ** -0.5 if scale is None else scale), _stream())
@@ -795,47 +816,47 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     axis in turn (``"cyclic"``).  Pair p is channels (p, p + rot/2)
     (``pairing="half"``) or (2p, 2p + 1) (``"adjacent"``).  q_weight / k_weight
     [D] fp32 scale the norm (None = 1); ``norm=False`` only rotates."""
-    _on_device(q, "q")
-    fmt = _HALF_FORMATS.get(q.dtype)
+    dev, dtype = _current_device(q, "q"), q.dtype
+    fmt = _HALF_FORMATS.get(dtype)
     if fmt is None:
-        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
-    _on_device(k, "k", q.dtype)
-    if q.dim() < 2 or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise TypeError(f"q must be fp16 or bf16, got {dtype}")
+    _on(dev, k, "k", dtype)
+    lead, D, Hq, Hk = q.shape[:-2], q.shape[-1], q.shape[-2], k.shape[-2]
+    if q.dim() < 3 or k.dim() != q.dim() or k.shape[:-2] != lead or k.shape[-1] != D:
         raise ValueError("q [..., Hq, D] and k [..., Hk, D] do not match")
-    lead, (Hq, D), Hk = q.shape[:-2], q.shape[-2:], k.shape[-2]
     N = lead.numel()
-    _on_device(inv_freq, "inv_freq", torch.float32)
+    _on(dev, inv_freq, "inv_freq", torch.float32)
     if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous vector")
     pairs = inv_freq.numel()
-    sections = (pairs,) if sections is None else tuple(int(x) for x in sections)
+    sections = (pairs,) if sections is None else tuple(sections)
     axes = len(sections)
-    _on_device(positions, "positions")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+    bits = _POSITION_BITS.get(positions.dtype) if isinstance(positions, torch.Tensor) else None
+    if bits is None:
+        raise TypeError("positions must be an int32 or int64 tensor")
+    _on(dev, positions, "positions", positions.dtype)
     if positions.shape != lead and positions.shape != (axes, *lead) or positions.numel() != axes * N:
         raise ValueError(f"positions must be {[*lead]} or {[axes, *lead]}")
     if not positions.is_contiguous():
         raise ValueError("positions must be contiguous")
     for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None:
-            _need(w, n, torch.float32)
-            if w.numel() != D:
-                raise ValueError(f"{n} must have D={D} elements")
+            _on(dev, w, n, torch.float32)
+            if w.shape != (D,) or not w.is_contiguous():
+                raise ValueError(f"{n} must hold D={D} contiguous values")
     outs = []
     for t, o, n in ((q, q_out, "q_out"), (k, k_out, "k_out")):
         if o is None:
-            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            o = t.new_empty(t.shape)
         else:
-            _on_device(o, n, t.dtype)
+            _on(dev, o, n, dtype)
             if o.shape != t.shape:
                 raise ValueError(f"{n} must be {[*t.shape]}")
         outs.append(o)
-    import ctypes
     _lib.call("cf_qk_norm_rope", q.data_ptr(), k.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(),
               fmt, N, Hq, Hk, D, *_head_strides(q, "q"), *_head_strides(k, "k"),
               *_head_strides(outs[0], "q_out"), *_head_strides(outs[1], "k_out"),
-              positions.data_ptr(), 32 if positions.dtype == torch.int32 else 64, N,
+              positions.data_ptr(), bits, N,
               inv_freq.data_ptr(), 2 * pairs, (ctypes.c_int32 * axes)(*sections), axes,
               _lookup(_AXIS_ORDERS, axis_order, "axis_order"), _lookup(_PAIRINGS, pairing, "pairing"),
               _ptr(q_weight), _ptr(k_weight), int(bool(norm)), float(eps), _stream())
