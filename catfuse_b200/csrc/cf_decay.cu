@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(1024) decay_segments_kernel(const int32_t* cu,
 }
 
 // A segment's own state L_r becomes the state that enters it:
-// E_0 = s_in (not stored), E_{r+1} = l^{seg_len} E_r + L_r.  One thread per four
-// entries of a (sequence, head); the states of a call fit the L2.
+// E_0 = s_in, E_{r+1} = l^{seg_len} E_r + L_r.  One thread per four entries of a
+// (sequence, head).
 __global__ void __launch_bounds__(256) decay_enter_kernel(const __grid_constant__ DecayArgs a,
                                                           const int32_t* first) {
   griddep_wait();
@@ -191,14 +191,18 @@ __global__ void __launch_bounds__(256) decay_enter_kernel(const __grid_constant_
   if (e >= dd) return;
   const int64_t r0 = a.segs ? first[seq] : seq * a.n_seg;
   const int n = a.segs ? first[seq + 1] - first[seq] : a.n_seg;
+  if (n < 2) return;
   const int64_t slot = a.slots ? a.slots[seq] : seq;
-  float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (a.s_in && slot >= 0 && slot < a.n_slots)
-    run = *reinterpret_cast<const float4*>(a.s_in + (slot * a.Hk + h) * dd + e);
-  const float2 l = pow_hi_lo(a.log_decay[h], a.seg_len);
+  const bool carried = a.s_in && slot >= 0 && slot < a.n_slots;
   const int64_t step = (int64_t)a.Hk * dd;
   float* p = a.seg_states + (r0 * a.Hk + h) * dd + e;
-  float4 own = n > 1 ? *reinterpret_cast<const float4*>(p) : run;
+  float4 own = *reinterpret_cast<const float4*>(p);
+  float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (carried) {
+    run = *reinterpret_cast<const float4*>(a.s_in + (slot * a.Hk + h) * dd + e);
+    *reinterpret_cast<float4*>(p) = run;
+  }
+  const float2 l = pow_hi_lo(a.log_decay[h], a.seg_len);
   for (int r = 1; r < n; ++r) {
     p += step;
     float4 next = own;
@@ -238,7 +242,8 @@ struct Plan {
 Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t Dv, bool packed, int sms) {
   Plan p{};
   const double t_walk = 1.0 + 0.7 * ((double)Hq / Hk - 1.0), t_sum = 0.6, t_cut = 8.0, t_unit = 3.0;
-  const int64_t units = S * Hk;
+  const bool narrow = Dk <= 64 && Dv <= 64;  // two walking CTAs an SM, three summing ones
+  const int64_t units = S * Hk, ctas = narrow ? 2 * sms : sms, ctas_s = narrow ? 3 * sms : sms;
   p.n_segs = S;
   p.n_seg = 1;
   p.seg_len = N > kC ? (N + kC - 1) / kC * kC : kC;
@@ -249,8 +254,8 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
       for (int64_t n = 1; n <= ch && n <= 256; ++n) {
         const int64_t len = (ch + n - 1) / n;
         if ((ch + len - 1) / len != n) continue;
-        const double waves = (double)((units * n + sms - 1) / sms);
-        const double waves_s = (double)((units * (n - 1) + sms - 1) / sms);
+        const double waves = (double)((units * n + ctas - 1) / ctas);
+        const double waves_s = (double)((units * (n - 1) + ctas_s - 1) / ctas_s);
         const double t = waves * (len * t_walk + t_unit) + (n > 1 ? waves_s * (len * t_sum + t_unit) + t_cut : 0.0);
         if (n == 1 || t < best) {
           best = t;
@@ -264,7 +269,7 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
       // Lengths are on the device.  The shorter the segments, the more evenly
       // they spread (half a segment is lost at the end), and the more of them
       // there are to set up: of c chunks for each CTA, c / len segments.
-      const double c = (double)(N / kC + S) * Hk / sms;
+      const double c = (double)(N / kC + S) * Hk / ctas;
       int64_t len = (int64_t)sqrt(2.0 * c * t_unit / t_walk) + 1;
       if (len < 4) len = 4;
       if (N > len * kC) {

@@ -23,7 +23,7 @@
 // zeros that TMA fills in.  With 128 of them V' and S^T go to the products from
 // TMEM, which halves what the products read from shared memory (the bound of
 // everything else that was tried: 128 bytes a cycle); with 64, an M = 64 product
-// takes them from shared memory.
+// takes them from shared memory and two CTAs share the SM.
 //
 // What is rounded to 16 bits on its way through a product, and how: V' carries
 // the state's precision, so it goes as three bf16 parts (24 bits) or two fp16
@@ -32,8 +32,8 @@
 // In fp16 every row of V', S and P is scaled by a power of two of its own, so that
 // neither a full state nor a small one leaves the type's range; bf16 has fp32's.
 //
-// Warpgroups: P (QK -> P), O (outputs), S (state), V (V'), and one with the TMA and
-// the MMA warp.
+// Warpgroups: P (QK -> P), O (outputs), S (state), V (V'; with 64 channels the S
+// warps do it), and one with the TMA and the MMA warp.
 #pragma once
 
 #include "cf_half.cuh"
@@ -165,10 +165,17 @@ __device__ __forceinline__ void tmem_wait16(float (&r)[16]) {
                  "+r"(u[7]), "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]),
                  "+r"(u[14]), "+r"(u[15])::"memory");
 }
-// 64 columns of two accumulators (of the first alone if !both), one wait.
-__device__ __forceinline__ void tmem_ld_pair(uint32_t ta, uint32_t tb, bool both, float (&x)[32], float (&y)[32]) {
+// 8 N columns of two accumulators (of the first alone if !both), one wait.
+template <int N>
+__device__ __forceinline__ void tmem_ld_pair(uint32_t ta, uint32_t tb, bool both, float (&x)[4 * N], float (&y)[4 * N]) {
   uint32_t* u = reinterpret_cast<uint32_t*>(x);
   uint32_t* v = reinterpret_cast<uint32_t*>(y);
+  if constexpr (N == 4) {
+    tmem_ld_frag4(ta, x);
+    if (both) tmem_ld_frag4(tb, y);
+    tmem_wait16(x);
+    tmem_wait16(y);
+  } else {
 #define CF_LD8(R, A)                                                                                              \
   asm volatile(                                                                                                   \
       "tcgen05.ld.sync.aligned.16x256b.x8.b32 "                                                                   \
@@ -184,14 +191,15 @@ __device__ __forceinline__ void tmem_ld_pair(uint32_t ta, uint32_t tb, bool both
   asm volatile(S : "+r"(R[O]), "+r"(R[O + 1]), "+r"(R[O + 2]), "+r"(R[O + 3]), "+r"(R[O + 4]), "+r"(R[O + 5]),    \
                    "+r"(R[O + 6]), "+r"(R[O + 7]), "+r"(R[O + 8]), "+r"(R[O + 9]), "+r"(R[O + 10]),               \
                    "+r"(R[O + 11]), "+r"(R[O + 12]), "+r"(R[O + 13]), "+r"(R[O + 14]), "+r"(R[O + 15])::"memory")
-  CF_LD8(u, ta);
-  if (both) CF_LD8(v, tb);
-  CF_WAIT16(u, 0, "tcgen05.wait::ld.sync.aligned;");
-  CF_WAIT16(u, 16, "");
-  CF_WAIT16(v, 0, "");
-  CF_WAIT16(v, 16, "");
+    CF_LD8(u, ta);
+    if (both) CF_LD8(v, tb);
+    CF_WAIT16(u, 0, "tcgen05.wait::ld.sync.aligned;");
+    CF_WAIT16(u, 16, "");
+    CF_WAIT16(v, 0, "");
+    CF_WAIT16(v, 16, "");
 #undef CF_LD8
 #undef CF_WAIT16
+  }
 }
 // 16 rows x 32 words of a packed 16-bit operand: thread t holds row t / 4, word
 // t % 4 of every four, then row t / 4 + 8 (the fragment above, packed in pairs).
@@ -389,20 +397,20 @@ template <typename T, int DK, int DV, bool OUT>
 struct Cfg {
   static constexpr bool kFp16 = std::is_same<T, __half>::value;
   static constexpr int kVParts = kFp16 ? 2 : 3;
-  static constexpr bool kTm = DV == 128;       // V' and S^T in TMEM
+  static constexpr bool kTm = DV == 128;       // V' and S^T in TMEM, V' by warps of its own
   static constexpr int kHalves = DV / 64;      // 16-row halves of a warp's lanes
   static constexpr int kCg = DK / 64;          // groups of 64 state columns
   // warpgroups
-  static constexpr int kP = 0, kO = OUT ? 1 : -1, kS = OUT ? 2 : 0, kV = kS + 1;
+  static constexpr int kP = 0, kO = OUT ? 1 : -1, kS = OUT ? 2 : 0, kV = kTm ? kS + 1 : kS;
   static constexpr int kCtl = kV + 1;
   static constexpr int kThreads = 128 * (kCtl + 1);
-  static constexpr int kCtas = DV == 64 && DK == 64 && !OUT ? 2 : 1;
+  static constexpr int kCtas = DV == 64 && DK == 64 ? (OUT ? 2 : 3) : 1;
   static constexpr int kKBytes = DK / 64 * kTileBytes;
   static constexpr int kVBytes = DV / 64 * kTileBytes;
   static constexpr int kSPart = DV * DK * 2;
-  static constexpr int kVp = (!OUT || (!kTm && DK == 64)) ? 2 : 1;  // V' and KV buffers
-  static constexpr int kKvStages = kCtas > 1 ? 3 : 4;
-  static constexpr int kQStages = OUT ? 4 : 0;
+  static constexpr int kVp = (!OUT && kTm) ? 2 : 1;  // V' and KV buffers
+  static constexpr int kKvStages = kCtas > 1 ? 2 : 4;
+  static constexpr int kQStages = OUT ? (kCtas > 1 ? 2 : 4) : 0;
   static constexpr int kScaleBytes = kFp16 ? 4096 : 0;
   static constexpr int kVpBytes = kTm ? 0 : kVp * kVParts * kVBytes;
   static constexpr int kSBytes = (OUT && !kTm) ? kSPart : 0;
@@ -415,10 +423,12 @@ struct Cfg {
   static constexpr int kColV = kColS + ((OUT && kTm) ? DK / 2 : 0);
   static constexpr int kColsUsed = kColV + (kTm ? kVp * kVParts * 32 : 0);
   static constexpr int kCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
-  // Registers of each warpgroup where the launch's even share (5 x 96) does not do.
-  static constexpr bool kMove = OUT;
-  static constexpr int kRegP = 96, kRegO = 96, kRegS = 168, kRegV = 96, kRegCtl = 24;
-  static_assert(!kMove || kRegP + kRegO + kRegS + kRegV + kRegCtl <= 5 * 96, "registers");
+  // Registers of each warpgroup where the launch's even share does not do
+  // (threads x registers at launch, over 128: 5 x 96 and 4 x 64).
+  static constexpr bool kMove = OUT && (kTm || kCtas == 2);
+  static constexpr int kRegP = kTm ? 96 : 80, kRegO = kTm ? (kFp16 ? 112 : 96) : 64, kRegS = kTm ? 168 : 88,
+                       kRegV = kFp16 ? 80 : 96, kRegCtl = 24;
+  static_assert(!kMove || kRegP + kRegO + kRegS + kRegCtl + (kTm ? kRegV : 0) <= (kTm ? 5 * 96 : 4 * 64), "registers");
 };
 
 struct Unit {
@@ -469,7 +479,10 @@ __device__ __forceinline__ bool get_unit(const DecayArgs& a, uint32_t u, Unit& x
   const int64_t slot = a.slots ? a.slots[x.seq] : x.seq;
   const bool has_slot = slot >= 0 && slot < a.n_slots;
   const int64_t row = (slot * a.Hk + x.h) * dd;
-  x.start = !first ? mine : (a.s_in && has_slot) ? a.s_in + row : nullptr;
+  // Where s_out is s_in, a sequence's last segment may be done before its first
+  // begins: several segments all start from their own copies.
+  const bool carried = a.s_in && has_slot;
+  x.start = !first || (carried && !last) ? mine : carried ? a.s_in + row : nullptr;
   x.end = (last && a.s_out && has_slot) ? a.s_out + row : nullptr;
   return true;
 }
@@ -793,6 +806,9 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
   } else if (OUT && wg == K::kP) {
     // ------------------------------------------------------------ QK -> P
     // Rows i = 16 wq + fr and + 8, columns j = 8 n + fc and + 1.
+    if constexpr (K::kMove) {
+      if constexpr (K::kRegP > (TM ? 96 : 64)) regs_up<K::kRegP>();
+    }
     if constexpr (OUT) {
       uint32_t it = 0;
       bool ok = true;
@@ -870,6 +886,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       if (!ok) give_up(ERR_SITE_DECAY_P, w);
     }
   } else if (OUT && wg == K::kO) {
+    if constexpr (K::kMove && K::kRegO > 96) regs_up<K::kRegO>();
     // ------------------------------------------------------------ outputs
     // Channels dv = (DV / 4) wq + 16 hh + fr and + 8, tokens 8 n + fc and + 1; put
     // out through shared memory as rows of a token.
@@ -896,12 +913,14 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           for (int g = 0; g < G; ++g, ++it) {
             if (!(ok = warp_wait(o_full, it & 1, w))) break;
             tc_fence_after();
-#pragma unroll 1
-            for (int hh = 0; hh < NH; ++hh) {  // 16 channels x 64 tokens
-              float p[32], z[32];
-              const uint32_t ta = tlane + ((uint32_t)(hh * 16) << 16);
-              tmem_ld_pair(ta + K::kColOp, ta + K::kColOs, has_s, p, z);
-              const bool last = hh == NH - 1;
+            // 16 channels x 64 tokens at a time; 32 tokens where registers are few
+            constexpr int NO = K::kCtas == 2 ? 4 : 8;
+            auto put = [&](int hh, auto half) {
+              constexpr int n0 = decltype(half)::value * NO;
+              float p[4 * NO], z[4 * NO];
+              const uint32_t ta = tlane + ((uint32_t)(hh * 16) << 16) + n0 * 8;
+              tmem_ld_pair<NO>(ta + K::kColOp, ta + K::kColOs, has_s, p, z);
+              const bool last = hh == NH - 1 && n0 + NO == 8;
               if (!FP16 && last) {
                 tc_fence_before();
                 warp_arrive(o_empty);
@@ -914,11 +933,11 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
                   ss[r] = pack2(e, e);
                 }
               }
-              uint32_t o[8][2];
+              uint32_t o[NO][2];
 #pragma unroll
-              for (int n = 0; n < 8; ++n) {
+              for (int n = 0; n < NO; ++n) {
                 F2 pf = 0;
-                if constexpr (FP16) pf = *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + 8 * n + fc]);
+                if constexpr (FP16) pf = *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + 8 * (n0 + n) + fc]);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                   F2 y = pack2(p[4 * n + 2 * r], p[4 * n + 2 * r + 1]);
@@ -926,7 +945,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
                   if (has_s) {
                     F2 x2 = pack2(z[4 * n + 2 * r], z[4 * n + 2 * r + 1]);
                     if constexpr (FP16) x2 = mul2(x2, ss[r]);
-                    y = fma2(grow[n], x2, y);
+                    y = fma2(grow[n0 + n], x2, y);
                   }
                   o[n][r] = Half2<T>::pack(y);
                 }
@@ -937,9 +956,14 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
               }
               // block m = lane / 8: tokens 8 (n + m / 2).., channels 8 (m % 2)..
 #pragma unroll
-              for (int n = 0; n < 8; n += 2)
-                stm4_t(stage_u + out_at<kRow>(8 * (n + (lane >> 4)) + (lane & 7), hh * 2 + ((lane >> 3) & 1)), o[n][0],
-                       o[n][1], o[n + 1][0], o[n + 1][1]);
+              for (int n = 0; n < NO; n += 2)
+                stm4_t(stage_u + out_at<kRow>(8 * (n0 + n + (lane >> 4)) + (lane & 7), hh * 2 + ((lane >> 3) & 1)),
+                       o[n][0], o[n][1], o[n + 1][0], o[n + 1][1]);
+            };
+#pragma unroll 1
+            for (int hh = 0; hh < NH; ++hh) {
+              put(hh, std::integral_constant<int, 0>{});
+              if constexpr (NO == 4) put(hh, std::integral_constant<int, 1>{});
             }
             if (s_badany[cc & 3] == cc + 1)
               spoil_outputs<kRow>(stage, s_bad + (cc & 3) * DV + wq * (DV / 4), cc);
@@ -1050,8 +1074,10 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             }
         };
         uint32_t part[K::kVParts][16];
-        split8(0, part, 0);
-        split8(8, part, 8);
+        if constexpr (TM) {
+          split8(0, part, 0);
+          split8(8, part, 8);
+        }
         // KV of the chunk before in this buffer has read its V'
         if (hh == 0) {
           if (!warp_wait(&ds_full[chunk % VP], ((chunk / VP) & 1) ^ 1, w)) return false;
@@ -1063,11 +1089,14 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             tmem_st_frag8(tlane + ((uint32_t)(hh * 16) << 16) + K::kColV + ((chunk % VP) * K::kVParts + q) * 32, part[q]);
         } else {
 #pragma unroll
-          for (int q = 0; q < K::kVParts; ++q) {
-            const uint32_t to = smem_u32(sVp) + ((chunk % VP) * K::kVParts + q) * K::kVBytes + (at - vu);
+          for (int h = 0; h < 16; h += 8) {
+            split8(h, part, 0);
 #pragma unroll
-            for (int z = 0; z < 4; ++z)
-              stm4_t(to + z * 2048, part[q][4 * z], part[q][4 * z + 1], part[q][4 * z + 2], part[q][4 * z + 3]);
+            for (int q = 0; q < K::kVParts; ++q) {
+              const uint32_t to = smem_u32(sVp) + q * K::kVBytes + (at - vu) + h * 512;
+              stm4_t(to, part[q][0], part[q][1], part[q][2], part[q][3]);
+              stm4_t(to + 2048, part[q][4], part[q][5], part[q][6], part[q][7]);
+            }
           }
         }
       }
@@ -1083,7 +1112,8 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       return true;
     };
 
-    if (wg == K::kV) {
+    if (TM && wg == K::kV) {
+      if constexpr (K::kMove && K::kRegV < 96) regs_down<K::kRegV>();
       uint32_t cc = 0;
       for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
@@ -1103,7 +1133,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
         if (!get_unit<OUT>(a, u, x)) continue;
-        const float ld = a.log_decay[x.h];
+        const float ld = a.log_decay[x.h], l2 = log2_decay(ld);
         const float2 whole = pow_hi_lo(ld, kC), tail = pow_hi_lo(ld, x.len & (kC - 1));
         const int64_t at = (int64_t)fc * a.Dv + dv0;
         if (x.start && a.Dk == DK && a.Dv == DV) {  // all loads in flight at once
@@ -1144,8 +1174,13 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
                 }
           }
         }
+        F2 f[8];
         for (int c = 0; c < x.len; c += kC, ++cc) {
           const int n = min(kC, x.len - c);
+          if constexpr (!TM) {  // before S, so that KV runs while S is put
+            if (c == 0 || n < kC) factors(l2, n, f);
+            if (!(ok = put_v(cc, n, f))) break;
+          }
           if (OUT && (c > 0 || x.start)) {
             // S^T in 16 bits, for the product with the queries; the one before it
             // is done when s_empty comes round
@@ -1260,7 +1295,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       }
     }
 
-    if (!ok) give_up(wg == K::kV ? ERR_SITE_DECAY_V : ERR_SITE_DECAY_STATE, w);
+    if (!ok) give_up(TM && wg == K::kV ? ERR_SITE_DECAY_V : ERR_SITE_DECAY_STATE, w);
   }
 
   tc_fence_before();

@@ -278,6 +278,32 @@ def test_long_prompts(dev, dtype, case):
     assert torch.equal(out, ops.decay_attention(q, k, v, ld, s_in=s2, s_out=s2)) and torch.equal(s, s2)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128), (128, 64), (64, 128)])
+@pytest.mark.parametrize("heads", [(8, 8), (16, 8)])
+def test_more_sequences_and_heads_than_fit_at_once(dev, dtype, dims, heads):
+    """Every CTA walks several (sequence, head) pairs, long and short by turns."""
+    from catfuse_b200 import ops
+    (dk, dv), (hq, hk) = dims, heads
+    g = torch.Generator().manual_seed(20)
+    lens = torch.randint(0, 400, (60,), generator=g)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]).to(torch.int32)
+    q, k, v = _make((int(cu[-1]),), hq, hk, dk, dv, dtype, 21)
+    ld = _log_decay(hk).to(dev)
+    s = torch.randn(60, hk, dk, dv, generator=g).to(dev)
+    s0 = s.clone()
+    out = ops.decay_attention(q, k, v, ld, s_in=s, s_out=s, cu_seqlens=cu.to(dev))
+    b = cu.tolist()
+    pick = [0, 1, 17, 36, 58, 59]  # the oracle is slow: every CTA's first and last pairs are among these
+    _check_sequences(q, k, v, ld, [(b[i], b[i + 1]) for i in pick], out, s0[pick], s[pick])
+    alone = torch.empty_like(s0)
+    for i in range(60):  # all of them against calls of their own
+        o = ops.decay_attention(q[b[i]:b[i + 1]][None], k[b[i]:b[i + 1]][None], v[b[i]:b[i + 1]][None], ld,
+                                s_in=s0[i:i + 1], s_out=alone[i:i + 1])
+        assert _close_16(out[b[i]:b[i + 1]], o[0])
+    assert (s - alone).norm() <= 2.0 ** -18 * alone.norm()
+
+
 def test_long_packed_prompts(dev):
     from catfuse_b200 import ops
     lens = [3000, 1, 0, 700, 64, 2111]
