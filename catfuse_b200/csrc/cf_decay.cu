@@ -196,24 +196,30 @@ __global__ void __launch_bounds__(256) decay_enter_kernel(const __grid_constant_
   const bool carried = a.s_in && slot >= 0 && slot < a.n_slots;
   const int64_t step = (int64_t)a.Hk * dd;
   float* p = a.seg_states + (r0 * a.Hk + h) * dd + e;
-  float4 own = *reinterpret_cast<const float4*>(p);
   float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (carried) {
-    run = *reinterpret_cast<const float4*>(a.s_in + (slot * a.Hk + h) * dd + e);
-    *reinterpret_cast<float4*>(p) = run;
+  if (carried) run = *reinterpret_cast<const float4*>(a.s_in + (slot * a.Hk + h) * dd + e);
+  // l^{seg_len}, its exponent kept to twice fp32's digits
+  const float len = (float)a.seg_len, x = a.log_decay[h] * len, rest = fmaf(a.log_decay[h], len, -x);
+  const float l = isfinite(x) ? expf(x) * (1.f + rest) : expf(x);
+  constexpr int kAhead = 4;  // own states in flight
+  for (int r = 0; r + 1 < n; r += kAhead) {
+    float4 own[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (r + i + 1 < n) own[i] = *reinterpret_cast<const float4*>(p + i * step);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (r + i + 1 < n) {
+        if (r + i > 0 || carried) *reinterpret_cast<float4*>(p + i * step) = run;
+        run.x = fmaf(l, run.x, own[i].x);
+        run.y = fmaf(l, run.y, own[i].y);
+        run.z = fmaf(l, run.z, own[i].z);
+        run.w = fmaf(l, run.w, own[i].w);
+      }
+    }
+    p += kAhead * step;
   }
-  const float2 l = pow_hi_lo(a.log_decay[h], a.seg_len);
-  for (int r = 1; r < n; ++r) {
-    p += step;
-    float4 next = own;
-    if (r + 1 < n) next = *reinterpret_cast<const float4*>(p);
-    run.x = fmaf(l.x, run.x, fmaf(l.y, run.x, own.x));
-    run.y = fmaf(l.x, run.y, fmaf(l.y, run.y, own.y));
-    run.z = fmaf(l.x, run.z, fmaf(l.y, run.z, own.z));
-    run.w = fmaf(l.x, run.w, fmaf(l.y, run.w, own.w));
-    *reinterpret_cast<float4*>(p) = run;
-    own = next;
-  }
+  *reinterpret_cast<float4*>(a.seg_states + ((r0 + n - 1) * a.Hk + h) * dd + e) = run;
 }
 
 // --------------------------------------------------------------------------
@@ -237,11 +243,11 @@ struct Plan {
 
 // How long the segments are.  Times in units of one chunk of a single query
 // head: the walk takes 1 for a chunk and its first query head and about 0.7 for
-// every further one, the pass that sums states 0.6; a segment costs 3 on top (its
+// every further one, the pass that sums states 0.6; a segment costs 5 on top (its
 // state comes and goes, its pipeline fills), a cut call's two more launches 8.
 Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t Dv, bool packed, int sms) {
   Plan p{};
-  const double t_walk = 1.0 + 0.7 * ((double)Hq / Hk - 1.0), t_sum = 0.6, t_cut = 8.0, t_unit = 3.0;
+  const double t_walk = 1.0 + 0.7 * ((double)Hq / Hk - 1.0), t_sum = 0.6, t_cut = 8.0, t_unit = 5.0;
   const bool narrow = Dk <= 64 && Dv <= 64;  // two walking CTAs an SM, three summing ones
   const int64_t units = S * Hk, ctas = narrow ? 2 * sms : sms, ctas_s = narrow ? 3 * sms : sms;
   p.n_segs = S;

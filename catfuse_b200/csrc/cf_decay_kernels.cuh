@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
                 tc_fence_before();
                 warp_arrive(o_empty);
               }
-              F2 ss[2];
+              [[maybe_unused]] F2 ss[2];
               if constexpr (FP16) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -936,7 +936,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
               uint32_t o[NO][2];
 #pragma unroll
               for (int n = 0; n < NO; ++n) {
-                F2 pf = 0;
+                [[maybe_unused]] F2 pf = 0;
                 if constexpr (FP16) pf = *reinterpret_cast<const F2*>(&s_pscale[(it & 1) * 64 + 8 * (n0 + n) + fc]);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {

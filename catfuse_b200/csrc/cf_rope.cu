@@ -29,7 +29,7 @@
 namespace cf {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 constexpr int kRopeMaxDim = 256;
 constexpr int kRopeMaxAxes = 4;
 

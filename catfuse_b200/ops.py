@@ -8,6 +8,7 @@ a CPU tensor or a missing library raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -737,6 +738,20 @@ def _decay_args(q, k, v, log_decay, out, dims):
     return dev, fmt, qs[-2], Hk, qs[-1], Dv, out
 
 
+@functools.lru_cache(maxsize=1024)
+def _decay_workspace(S, N, Hq, Hk, Dk, Dv, packed, device) -> int:
+    """Workspace bytes: they depend on the sizes and the (current) device alone."""
+    need = _lib.load().cf_decay_attention_workspace(S, N, Hq, Hk, Dk, Dv, packed)
+    if need < 0:
+        _lib.check(need, "cf_decay_attention_workspace")
+    return need
+
+
+@functools.lru_cache(maxsize=256)
+def _section_array(sections):
+    return (ctypes.c_int32 * len(sections))(*sections)
+
+
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
                     scale: Optional[float] = None, s_in: Optional[torch.Tensor] = None,
                     s_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
@@ -765,9 +780,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     if len(rows) == 2 and rows[0] != rows[1]:
         raise ValueError("s_in and s_out must have the same number of rows")
     slots_ptr = _slots(dev, slots, S)
-    need = _lib.load().cf_decay_attention_workspace(S, N, Hq, Hk, Dk, Dv, packed)
-    if need < 0:
-        _lib.check(need, "cf_decay_attention_workspace")
+    need = _decay_workspace(S, N, Hq, Hk, Dk, Dv, packed, dev.index)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.call("cf_decay_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), fmt,
               log_decay.data_ptr(), _ptr(s_in), _ptr(s_out), slots_ptr, rows[0] if rows else 0,
@@ -857,7 +870,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
               fmt, N, Hq, Hk, D, *_head_strides(q, "q"), *_head_strides(k, "k"),
               *_head_strides(outs[0], "q_out"), *_head_strides(outs[1], "k_out"),
               positions.data_ptr(), bits, N,
-              inv_freq.data_ptr(), 2 * pairs, (ctypes.c_int32 * axes)(*sections), axes,
+              inv_freq.data_ptr(), 2 * pairs, _section_array(sections), axes,
               _lookup(_AXIS_ORDERS, axis_order, "axis_order"), _lookup(_PAIRINGS, pairing, "pairing"),
               _ptr(q_weight), _ptr(k_weight), int(bool(norm)), float(eps), _stream())
     return tuple(outs)

@@ -449,14 +449,14 @@ CF_API int cf_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_ou
 
 /* ---- bounded device-side waits ------------------------------------------- */
 
-/* Every mbarrier wait inside the fused conv kernel gives up after a bounded
- * number of polls, records a site code in the device error word
+/* Every mbarrier wait inside the fused conv kernel and the prompt kernel of
+ * cf_decay_attention gives up after a bounded number of polls, records a site code in the device error word
  * (cf_check_device_error) and ends the kernel early.  This sets that bound for
  * later launches in this process (0 = the default, 2^24 polls, i.e. seconds).
  * The reference has no counterpart (Triton kernels there have no waits). */
 CF_API int cf_set_wait_limit(uint32_t max_polls);
-/* Test hook for that expiry path: when armed, the next cf_conv_bn_lif launch
- * has CTA 0's producers skip their first load, so the consumer's wait for it
+/* Test hook for that expiry path: when armed, the next cf_conv_bn_lif or
+ * tensor-core cf_decay_attention call has CTA 0's producers skip their first load, so the consumer's wait for it
  * runs out; the kernel ends early and cf_check_device_error reports
  * CF_ERR_DEVICE_TIMEOUT.  One-shot (disarmed by that launch); 0 disarms. */
 CF_API int cf_test_arm_stalled_load(int armed);

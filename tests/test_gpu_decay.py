@@ -408,6 +408,28 @@ def test_offsets_beyond_32_bits(dev):
     _check_state(pool[rows - 1], S, aS)
 
 
+def test_a_wait_that_runs_out_is_reported(dev):
+    """One CTA's first load is left out: its waits give up within their limit, the
+    host learns of it, and the next call is as ever."""
+    from catfuse_b200 import _lib, ops
+    q, k, v = _make((1, 200), 2, 2, 64, 64, torch.float16, 22)
+    ld = _log_decay(2, "-0.1").to(dev)
+    want = ops.decay_attention(q, k, v, ld)
+    ops.check_device_error()
+    ops.set_wait_limit(2000)
+    try:
+        _lib.call("cf_test_arm_stalled_load", 1)
+        ops.decay_attention(q, k, v, ld)
+        with pytest.raises(_lib.CatfuseNativeError) as e:
+            ops.check_device_error()
+        assert e.value.code == _lib.CF_ERR_DEVICE_TIMEOUT
+    finally:
+        _lib.call("cf_test_arm_stalled_load", 0)
+        ops.set_wait_limit(0)
+    assert torch.equal(ops.decay_attention(q, k, v, ld), want)
+    ops.check_device_error()
+
+
 def test_nothing_to_do(dev):
     from catfuse_b200 import ops
     z = torch.empty(0, 5, 2, 64, dtype=torch.float16, device=dev)
