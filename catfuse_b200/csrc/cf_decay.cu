@@ -248,8 +248,7 @@ struct Plan {
 Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t Dv, bool packed, int sms) {
   Plan p{};
   const double t_walk = 1.0 + 0.7 * ((double)Hq / Hk - 1.0), t_sum = 0.6, t_cut = 8.0, t_unit = 5.0;
-  const bool narrow = Dk <= 64 && Dv <= 64;  // two walking CTAs an SM, three summing ones
-  const int64_t units = S * Hk, ctas = narrow ? 2 * sms : sms, ctas_s = narrow ? 3 * sms : sms;
+  const int64_t units = S * Hk, ctas = (Dk <= 64 && Dv <= 64) ? 2 * sms : sms;
   p.n_segs = S;
   p.n_seg = 1;
   p.seg_len = N > kC ? (N + kC - 1) / kC * kC : kC;
@@ -261,7 +260,7 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
         const int64_t len = (ch + n - 1) / n;
         if ((ch + len - 1) / len != n) continue;
         const double waves = (double)((units * n + ctas - 1) / ctas);
-        const double waves_s = (double)((units * (n - 1) + ctas_s - 1) / ctas_s);
+        const double waves_s = (double)((units * (n - 1) + ctas - 1) / ctas);
         const double t = waves * (len * t_walk + t_unit) + (n > 1 ? waves_s * (len * t_sum + t_unit) + t_cut : 0.0);
         if (n == 1 || t < best) {
           best = t;

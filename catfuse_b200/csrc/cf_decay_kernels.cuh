@@ -401,15 +401,15 @@ struct Cfg {
   static constexpr int kHalves = DV / 64;      // 16-row halves of a warp's lanes
   static constexpr int kCg = DK / 64;          // groups of 64 state columns
   // warpgroups
-  static constexpr int kP = 0, kO = OUT ? 1 : -1, kS = OUT ? 2 : 0, kV = kTm ? kS + 1 : kS;
+  static constexpr int kP = 0, kO = OUT ? 1 : -1, kS = OUT ? 2 : 0, kV = (kTm || !OUT) ? kS + 1 : kS;
   static constexpr int kCtl = kV + 1;
   static constexpr int kThreads = 128 * (kCtl + 1);
-  static constexpr int kCtas = DV == 64 && DK == 64 ? (OUT ? 2 : 3) : 1;
+  static constexpr int kCtas = DV == 64 && DK == 64 ? 2 : 1;
   static constexpr int kKBytes = DK / 64 * kTileBytes;
   static constexpr int kVBytes = DV / 64 * kTileBytes;
   static constexpr int kSPart = DV * DK * 2;
-  static constexpr int kVp = (!OUT && kTm) ? 2 : 1;  // V' and KV buffers
-  static constexpr int kKvStages = kCtas > 1 ? 2 : 4;
+  static constexpr int kVp = OUT ? 1 : 2;  // V' and KV buffers
+  static constexpr int kKvStages = kCtas == 1 ? 4 : OUT ? 2 : 3;
   static constexpr int kQStages = OUT ? (kCtas > 1 ? 2 : 4) : 0;
   static constexpr int kScaleBytes = kFp16 ? 4096 : 0;
   static constexpr int kVpBytes = kTm ? 0 : kVp * kVParts * kVBytes;
@@ -1093,7 +1093,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             split8(h, part, 0);
 #pragma unroll
             for (int q = 0; q < K::kVParts; ++q) {
-              const uint32_t to = smem_u32(sVp) + q * K::kVBytes + (at - vu) + h * 512;
+              const uint32_t to = smem_u32(sVp) + ((chunk % VP) * K::kVParts + q) * K::kVBytes + (at - vu) + h * 512;
               stm4_t(to, part[q][0], part[q][1], part[q][2], part[q][3]);
               stm4_t(to + 2048, part[q][4], part[q][5], part[q][6], part[q][7]);
             }
@@ -1112,7 +1112,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       return true;
     };
 
-    if (TM && wg == K::kV) {
+    if (K::kV != K::kS && wg == K::kV) {
       if constexpr (K::kMove && K::kRegV < 96) regs_down<K::kRegV>();
       uint32_t cc = 0;
       for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
@@ -1177,7 +1177,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         F2 f[8];
         for (int c = 0; c < x.len; c += kC, ++cc) {
           const int n = min(kC, x.len - c);
-          if constexpr (!TM) {  // before S, so that KV runs while S is put
+          if constexpr (K::kV == K::kS) {  // before S, so that KV runs while S is put
             if (c == 0 || n < kC) factors(l2, n, f);
             if (!(ok = put_v(cc, n, f))) break;
           }
