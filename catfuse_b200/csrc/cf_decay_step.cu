@@ -9,6 +9,9 @@
 // A CTA takes 32 columns of one state: eight lanes cover a row's 128 bytes, so
 // every request is whole sectors, and columns are independent, so no sums cross
 // CTAs and the result does not depend on the grid.
+//
+// Measured: 128 sequences of 32 states of 128 x 128, 94 us = 5.7 TB/s, 0.87 of the
+// measured copy bandwidth; 61 of 8 states (64 MB, which the L2 holds) 18 us.
 #include "cf_half.cuh"
 
 namespace cf {

@@ -407,8 +407,10 @@ CF_API int cf_pack_conv_weight_planes(const float* w, void* wq, int64_t Cout, in
  * sequence among n_slots rows; a slot outside [0, n_slots) starts from zeros
  * and stores nothing.  Rows of one call must differ.
  * `workspace`: cf_decay_attention_workspace bytes, 16-byte aligned, free for
- * reuse once the call's kernels have run.  A non-finite v reaches the outputs of
- * its own sequence only. */
+ * reuse once the call's kernels have run.  A non-finite value reaches outputs of
+ * its own sequence only, from its own token on (as infinity or NaN).  Rows of q, k and
+ * v on 16-byte boundaries (address and strides) run on the tensor cores; other
+ * rows take a plain recurrence. */
 CF_API int64_t cf_decay_attention_workspace(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk,
                                             int64_t Dv, int packed);
 CF_API int cf_decay_attention(const void* q, const void* k, const void* v, void* out, int fmt,

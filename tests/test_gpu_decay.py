@@ -304,6 +304,21 @@ def test_more_sequences_and_heads_than_fit_at_once(dev, dtype, dims, heads):
     assert (s - alone).norm() <= 2.0 ** -18 * alone.norm()
 
 
+def test_overlapping_boundaries_stay_in_bounds(dev):
+    """Boundaries that do not ascend are the caller's error: outputs of the
+    sequences concerned mean nothing, but nothing outside them is touched."""
+    from catfuse_b200 import ops
+    n = 3000
+    q, k, v = _make((n + 64,), 1, 1, 64, 64, torch.float16, 23)
+    ld = _log_decay(1, "-0.1").to(dev)
+    cu = torch.tensor([0, n] * 20 + [0], dtype=torch.int32, device=dev)
+    out = torch.full_like(v, 7.0)
+    s = torch.full((41, 1, 64, 64), 5.0, device=dev)
+    ops.decay_attention(q, k, v, ld, s_out=s[:40], cu_seqlens=cu, out=out)
+    torch.cuda.synchronize()
+    assert (out[n:] == 7).all() and (s[40] == 5).all()
+
+
 def test_long_packed_prompts(dev):
     from catfuse_b200 import ops
     lens = [3000, 1, 0, 700, 64, 2111]
