@@ -10,16 +10,18 @@
 // every request is whole sectors, and columns are independent, so no sums cross
 // CTAs and the result does not depend on the grid.
 //
-// Measured: 128 sequences of 32 states of 128 x 128, 94 us = 5.7 TB/s, 0.87 of the
-// measured copy bandwidth; 61 of 8 states (64 MB, which the L2 holds) 18 us.
+// Measured: 128 sequences of 32 states of 128 x 128, 85 us = 6.4 TB/s, 0.97 of the
+// measured copy bandwidth (256 threads with half the rows each: 90 us, 64 with twice
+// as many: 89 us); 512 sequences of 64 x 64, 98 us of a floor of 83 (130 with 256).
 #include "cf_half.cuh"
 
 namespace cf {
 namespace {
 
-constexpr int kStepThreads = 256;
+constexpr int kStepThreads = 128;
 constexpr int kStepCols = 32;   // state columns of a CTA
 constexpr int kStepMaxDim = 128;
+static_assert(kStepThreads >= kStepMaxDim, "a thread loads one entry of q and k");
 constexpr int kStepRowGroups = kStepThreads / (kStepCols / 4);
 constexpr int kStepRows = kStepMaxDim / kStepRowGroups;  // state rows of a thread
 
