@@ -421,6 +421,11 @@ struct Cfg {
   static constexpr int kVBytes = DV / 64 * kTileBytes;
   static constexpr int kSPart = DV * DK * 2;
   static constexpr int kVp = OUT ? 1 : 2;  // V' and KV buffers
+  // Chunks whose V' scales (fp16) are held.  V writes those of chunk c before it waits for a
+  // buffer of V': KV of chunk c - kVp - 1 is done by then, so S has let go of the accumulator
+  // of c - 2 kVp - 1, but may still read its last scales.  That takes 2 kVp + 2 slots.
+  static constexpr int kVScales = OUT ? 4 : 8;
+  static_assert(kVScales >= 2 * kVp + 2, "slots of V' scales");
   static constexpr int kKvStages = kCtas == 1 ? 4 : OUT ? 2 : 3;
   static constexpr int kQStages = OUT ? (kCtas > 1 ? 2 : 4) : 0;
   static constexpr int kScaleBytes = kFp16 ? 4096 : 0;
@@ -562,8 +567,10 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
   uint8_t* sP = sS + K::kSBytes;
   uint8_t* sOut = sP + (OUT ? kTileBytes : 0);
   float* s_sscale = reinterpret_cast<float*>(sOut + K::kStage);  // fp16 only: [2][128] S's scales by chunk,
-  float* s_pscale = s_sscale + 256;                              // [2][64] P's by item,
-  float* s_vscale = s_pscale + 128;                              // [4][128] V's by chunk
+  float* s_pscale = s_sscale + (OUT ? 256 : 0);                  // [2][64] P's by item (both in the walk),
+  float* s_vscale = s_pscale + (OUT ? 128 : 0);                  // [kVScales][128] V's by chunk
+  static_assert(!FP16 || ((OUT ? 384 : 0) + K::kVScales * 128) * 4 <= K::kScaleBytes, "scales");
+  constexpr uint32_t kVMask = K::kVScales - 1;
   uint8_t* small = sOut + K::kStage + K::kScaleBytes;
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(small);
   uint64_t* kv_empty = kv_full + 4;
@@ -1067,7 +1074,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             m = min(max(m & 0xFFFFu, m >> 16), 0x7BFFu);
             const int e = fp16_shift(__half2float(__ushort_as_half((unsigned short)m)));
             up[r] = pow2i(e);
-            if ((lane & 3) == 0) s_vscale[(chunk & 3) * 128 + d0 + fr + 8 * r] = pow2i(-e);
+            if ((lane & 3) == 0) s_vscale[(chunk & kVMask) * 128 + d0 + fr + 8 * r] = pow2i(-e);
           }
         }
         auto split8 = [&](int h, uint32_t (*part)[16], int o) {
@@ -1272,8 +1279,8 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             const int hh = q / (2 * K::kCg);
             float dn[2] = {1.f, 1.f};
             if constexpr (FP16) {
-              dn[0] = s_vscale[(cc & 3) * 128 + dv0 + hh * 16];
-              dn[1] = s_vscale[(cc & 3) * 128 + dv0 + hh * 16 + 8];
+              dn[0] = s_vscale[(cc & kVMask) * 128 + dv0 + hh * 16];
+              dn[1] = s_vscale[(cc & kVMask) * 128 + dv0 + hh * 16 + 8];
             }
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
