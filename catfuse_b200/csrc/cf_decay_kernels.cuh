@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
   uint8_t* sS = sVp + K::kVpBytes;
   uint8_t* sP = sS + K::kSBytes;
   uint8_t* sOut = sP + (OUT ? kTileBytes : 0);
-  float* s_sscale = reinterpret_cast<float*>(sOut + K::kStage);  // fp16 only: [2][128] S's scales by chunk,
+  float* s_sscale = reinterpret_cast<float*>(sOut + K::kStage);  // fp16 only: [2][128] S's scales by put,
   float* s_pscale = s_sscale + (OUT ? 256 : 0);                  // [2][64] P's by item (both in the walk),
   float* s_vscale = s_pscale + (OUT ? 128 : 0);                  // [kVScales][128] V's by chunk
   static_assert(!FP16 || ((OUT ? 384 : 0) + K::kVScales * 128) * 4 <= K::kScaleBytes, "scales");
@@ -910,7 +910,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
     // Channels dv = (DV / 4) wq + 16 hh + fr and + 8, tokens 8 n + fc and + 1; put
     // out through shared memory as rows of a token.
     if constexpr (OUT) {
-      uint32_t it = 0, cc = 0;
+      uint32_t it = 0, cc = 0, ns = 0;
       bool ok = true;
       constexpr int kRow = DV / 4 * 2;       // bytes of a token's row of this warp: 64 or 32
       constexpr int kVec = kRow / 16;        // 16-byte vectors of it
@@ -948,7 +948,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
               if constexpr (FP16) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                  const float e = s_sscale[(cc & 1) * 128 + wq * (DV / 4) + hh * 16 + fr + 8 * r];
+                  const float e = s_sscale[(ns & 1) * 128 + wq * (DV / 4) + hh * 16 + fr + 8 * r];
                   ss[r] = pack2(e, e);
                 }
               }
@@ -1006,6 +1006,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
             }
             __syncwarp();
           }
+          ns += has_s;
         }
       }
       if (!ok) give_up(ERR_SITE_DECAY_O, w);
@@ -1202,7 +1203,10 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
           }
           if (OUT && (c > 0 || x.start)) {
             // S^T in 16 bits, for the product with the queries; the one before it
-            // is done when s_empty comes round
+            // is done when s_empty comes round.  The scales' slots go by puts: the product
+            // with put ns - 1 was issued after the O warps were done with put ns - 2, whose
+            // slot this is.  By chunks nothing would order the two, since a chunk that
+            // starts from zeros puts no S.
             if (!(ok = warp_wait(s_empty, (ns & 1) ^ 1, w))) break;
             tc_fence_after();
 #pragma unroll
@@ -1224,7 +1228,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
                   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                   const int e = fp16_shift(m);
                   up[r] = pow2i(e);
-                  if ((lane & 3) == 0) s_sscale[(cc & 1) * 128 + dv0 + hh * 16 + 8 * r] = pow2i(-e);
+                  if ((lane & 3) == 0) s_sscale[(ns & 1) * 128 + dv0 + hh * 16 + 8 * r] = pow2i(-e);
                 }
               }
 #pragma unroll

@@ -63,3 +63,42 @@ def test_segment_sums_of_one_long_prompt(dev, dims):
     o, S, ao, aS = chunked(q, k, v, ld, s_in=s0[0])
     check_out(out[0], o, ao)
     check_state(s1[0], S, aS)
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("states", ["none", "some", "all"])
+def test_units_that_start_from_zeros(dev, dims, aligned, states):
+    """More (sequence, head) pairs than CTAs, long and short, where all, some or none
+    begin with a state; neighbours differ in size by up to 2^6."""
+    from catfuse_b200 import ops
+    dk, dv = dims
+    h, n_seq = 8, 64
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(60, 400, (n_seq,), generator=g).tolist()
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    b = cu.tolist()
+    q, k, v = _inputs(b[-1], h, h, dk, dv, 6, dev)
+    for i in range(n_seq):
+        v[b[i]:b[i + 1]] *= 2.0 ** (i * 3 % 7)
+    q, k, v = q.half(), k.half(), v.half()
+    ld = _decays(h, dev)
+    pool = 30.0 * torch.randn(n_seq, h, dk, dv, generator=g).to(dev)
+    slots = torch.arange(n_seq, dtype=torch.int32)
+    if states == "some":
+        slots[torch.rand(n_seq, generator=g) < 0.6] = -1
+    s_in = None if states == "none" else pool
+    s_out = torch.zeros_like(pool)
+    wide = torch.zeros(b[-1], h, dv + (0 if aligned else 3), dtype=torch.float16, device=dev)
+    ops.decay_attention(q, k, v, ld, s_in=s_in, s_out=s_out, slots=slots.to(dev), cu_seqlens=cu.to(dev),
+                        out=wide[..., :dv])
+    for i in range(n_seq):
+        part = slice(b[i], b[i + 1])
+        held = s_in is not None and slots[i] >= 0
+        o, S, ao, aS = chunked(q[part], k[part], v[part], ld, s_in=pool[i] if held else None)
+        check_out(wide[part, :, :dv], o, ao, f"sequence {i}")
+        if slots[i] >= 0:
+            check_state(s_out[i], S, aS, f"state {i}")
+        else:
+            assert (s_out[i] == 0).all()
+    assert (wide[..., dv:] == 0).all()
