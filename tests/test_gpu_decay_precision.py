@@ -1,0 +1,30 @@
+"""States stay within 2^-18 of their terms where that is hardest: slow decays over
+many segments, steep ones over large early values and silent tails."""
+import pytest
+import torch
+
+from decay_parity import HALF, check_out, check_state, chunked
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("log_decay", [-1.7e-7, -7e-7, -1e-6, -1e-5])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128)])
+def test_carried_state_over_many_segments(dev, dtype, log_decay, packed, dims):
+    from catfuse_b200 import ops
+    (dk, dv), n = dims, 16384
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, k, v = [(torch.randn(n, 1, d, generator=g, device=dev) / 64).to(dtype) for d in (dk, dk, dv)]
+    ld = torch.tensor([log_decay], device=dev)
+    s0 = 16.0 * torch.randn(1, 1, dk, dv, generator=g, device=dev)
+    s1 = torch.empty_like(s0)
+    if packed:
+        out = ops.decay_attention(q, k, v, ld, s_in=s0, s_out=s1,
+                                  cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device=dev))
+    else:
+        out = ops.decay_attention(q[None], k[None], v[None], ld, s_in=s0, s_out=s1)[0]
+    o, S, ao, aS = chunked(q, k, v, ld, s_in=s0[0])
+    check_out(out, o, ao)
+    check_state(s1[0], S, aS)
