@@ -397,6 +397,18 @@ __device__ __forceinline__ float log2_decay(float log_decay) {
   const float l2 = log_decay * 1.4426950408889634f;
   return l2 < -1e4f ? -1e4f : l2;
 }
+// The factors of V' reach the state: l^d for 0 <= d < 64 within 2^-21.  log2(l) stands as
+// hi + lo, since one rounding of an exponent near 100 alone is 2^-18 of the power.
+__device__ __forceinline__ float2 log2_decay_hi_lo(float log_decay) {
+  const float hi = log_decay * 1.4426950408889634f;
+  if (!(hi >= -1e4f)) return make_float2(hi < -1e4f ? -1e4f : hi, 0.f);
+  return make_float2(hi, fmaf(log_decay, 1.925963e-8f, fmaf(log_decay, 1.4426950408889634f, -hi)));
+}
+__device__ __forceinline__ float decay_power(float2 l2, float d) {
+  const float x = l2.x * d, rest = fmaf(l2.y, d, fmaf(l2.x, d, -x));
+  const float p = exp2_fast(x);
+  return fmaf(p, rest * 0.69314718f, p);
+}
 // l^n as hi + lo, for the factor that a state meets chunk after chunk.
 __device__ __forceinline__ float2 pow_hi_lo(float log_decay, int64_t n) {
   if (n == 0) return make_float2(1.f, 0.f);
@@ -1019,11 +1031,11 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
 
     // V' of chunk `chunk` (n tokens): v comes transposed from its tile (rows dv,
     // tokens 8 m + fc and + 1), meets f (l^{n-1-j}), and goes out in parts.
-    auto factors = [&](float l2, int n, F2 (&f)[8]) {
+    auto factors = [&](float2 l2, int n, F2 (&f)[8]) {
 #pragma unroll
       for (int m = 0; m < 8; ++m) {
         const int d = n - 1 - 8 * m - fc;
-        f[m] = pack2(d < 0 ? 0.f : exp2_fast(l2 * (float)d), d < 1 ? 0.f : exp2_fast(l2 * (float)(d - 1)));
+        f[m] = pack2(d < 0 ? 0.f : decay_power(l2, (float)d), d < 1 ? 0.f : decay_power(l2, (float)(d - 1)));
       }
     };
     auto put_v = [&](uint32_t chunk, int n, const F2 (&f)[8]) -> bool {
@@ -1138,7 +1150,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
         if (!get_unit<OUT>(a, u, x)) continue;
-        const float l2 = log2_decay(a.log_decay[x.h]);
+        const float2 l2 = log2_decay_hi_lo(a.log_decay[x.h]);
         F2 f[8];
         for (int c = 0; c < x.len && ok; c += kC, ++cc) {
           const int n = min(kC, x.len - c);
@@ -1153,7 +1165,8 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       for (uint32_t u = blockIdx.x; u < a.n_units && ok; u += gridDim.x) {
         Unit x;
         if (!get_unit<OUT>(a, u, x)) continue;
-        const float ld = a.log_decay[x.h], l2 = log2_decay(ld);
+        const float ld = a.log_decay[x.h];
+        const float2 l2 = log2_decay_hi_lo(ld);
         const float2 whole = pow_hi_lo(ld, kC), tail = pow_hi_lo(ld, x.len & (kC - 1));
         const int64_t at = (int64_t)fc * a.Dv + dv0;
         if (x.start && a.Dk == DK && a.Dv == DV) {  // all loads in flight at once

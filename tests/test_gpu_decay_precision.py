@@ -28,3 +28,22 @@ def test_carried_state_over_many_segments(dev, dtype, log_decay, packed, dims):
     o, S, ao, aS = chunked(q, k, v, ld, s_in=s0[0])
     check_out(out, o, ao)
     check_state(s1[0], S, aS)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("n", [64, 50, 128])
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128)])
+def test_silent_tail_under_steep_decays(dev, dtype, n, dims):
+    """Only the first token of each chunk speaks: what is left of it is its decay's power."""
+    from catfuse_b200 import ops
+    (dk, dv), h = dims, 48
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, v = [torch.randn(n, h, d, generator=g, device=dev) for d in (dk, dk, dv)]
+    for t in (k, v):
+        t *= (torch.arange(n, device=dev) % 64 == 0)[:, None, None]
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    ld = -torch.linspace(0.3, 1.2, h, device=dev)
+    s = torch.empty(1, h, dk, dv, device=dev)
+    ops.decay_attention(q[None], k[None], v[None], ld, s_out=s)
+    _, S, _, aS = chunked(q, k, v, ld)
+    check_state(s[0], S, aS)
