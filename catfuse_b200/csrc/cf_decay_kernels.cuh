@@ -31,7 +31,8 @@
 // parts (22 bits).  S and P reach only the 16-bit outputs and are rounded once,
 // which makes the outputs' error 1.42 times that of their own rounding alone.
 // In fp16 every row of V', S and P is scaled by a power of two of its own, so that
-// neither a full state nor a small one leaves the type's range; bf16 has fp32's.
+// neither a full state nor a small one leaves the type's range; bf16 has fp32's.  A term of V'
+// below 2^-17 of its row's largest is held to 2^-39 of that.
 //
 // Warpgroups: P (QK -> P), O (outputs), S (state), V (V'; in the walk with 64 channels
 // the S warps do it), and one with the TMA and the MMA warp.
@@ -1077,15 +1078,53 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
         odd = odd || max(top & 0xFFFFu, top >> 16) >= Half2<T>::kInf;
         float up[2] = {1.f, 1.f};
         if constexpr (FP16) {
+          // Row scales come from the largest |V'|, not |v|: under a steep decay the largest v
+          // may be all but gone.  Where the S warps do this (64 channels: the longest
+          // chain), products in fp16 do for most rows: they are off by 2^-9 at most
+          // (factors and results below 2^-14), a quarter of 2^-7; only rows below that take
+          // fp32.  (65536 tokens of 16 heads of 64: 240 us; 269 with fp32 everywhere, 256 with
+          // fp16 first everywhere, which took 128 channels from 104 to 117.)
+          float m[2];
+          bool small = true;
+          if constexpr (K::kV == K::kS) {
+            uint32_t live[2] = {0, 0};
+            __half2 p[2] = {__half2(), __half2()};
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const uint32_t fu = Half2<__half>::pack(f[y]);
+              const __half2 fh = *reinterpret_cast<const __half2*>(&fu);
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                live[r] |= raw[2 * y + r];
+                p[r] = __hmax2(p[r], __habs2(__hmul2(*reinterpret_cast<const __half2*>(&raw[2 * y + r]), fh)));
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              p[r] = __hmax2(p[r], __shfl_xor_sync(0xffffffffu, p[r], 1));
+              p[r] = __hmax2(p[r], __shfl_xor_sync(0xffffffffu, p[r], 2));
+              m[r] = fmaxf(__low2float(p[r]), __high2float(p[r]));
+            }
+            small = __any_sync(0xffffffffu, (m[0] < 0x1p-7f && (live[0] & 0x7FFF7FFFu)) ||
+                                                (m[1] < 0x1p-7f && (live[1] & 0x7FFF7FFFu)));
+          }
+          if (small) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              m[r] = 0.f;
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                float a0, a1;
+                unpack2(mul2(Half2<T>::unpack(raw[2 * y + r]), f[y]), a0, a1);
+                m[r] = fmaxf(m[r], fmaxf(fabsf(a0), fabsf(a1)));
+              }
+              m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
+              m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2));
+            }
+          }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int y = 0; y < 8; ++y) m = __vmaxu2(m, raw[2 * y + r] & 0x7FFF7FFFu);
-            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            m = min(max(m & 0xFFFFu, m >> 16), 0x7BFFu);
-            const int e = fp16_shift(__half2float(__ushort_as_half((unsigned short)m)));
+            const int e = fp16_shift(m[r]);
             up[r] = pow2i(e);
             if ((lane & 3) == 0) s_vscale[(chunk & kVMask) * 128 + d0 + fr + 8 * r] = pow2i(-e);
           }
