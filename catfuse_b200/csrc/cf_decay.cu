@@ -67,12 +67,13 @@ __global__ void __launch_bounds__(kThreads) decay_recurrent_kernel(const __grid_
   const int c = slice * kCols + lane;
   const bool on = c < a.Dv;
   const float2 decay = decay_hi_lo(a.log_decay[h]);
+  const bool carried = a.s_in && has_slot && (t0 == t1 || keeps_state(a.log_decay[h]));
   const int64_t base = (slot * a.Hk + h) * a.Dk * a.Dv + c;
   float s[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int r = i * kWarps + warp;
-    s[i] = (on && r < a.Dk && a.s_in && has_slot) ? a.s_in[base + (int64_t)r * a.Dv] : 0.f;
+    s[i] = (on && r < a.Dk && carried) ? a.s_in[base + (int64_t)r * a.Dv] : 0.f;
   }
   for (int64_t t = t0; t < t1; t += kTok) {
     const int n = t1 - t < kTok ? (int)(t1 - t) : kTok;
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(256) decay_enter_kernel(const __grid_constant_
   const int64_t step = (int64_t)a.Hk * dd;
   float* p = a.seg_states + (r0 * a.Hk + h) * dd + e;
   double run[4] = {0.0, 0.0, 0.0, 0.0};
-  if (carried) {
+  if (carried && keeps_state(a.log_decay[h])) {
     const float4 x = *reinterpret_cast<const float4*>(a.s_in + (slot * a.Hk + h) * dd + e);
     run[0] = x.x, run[1] = x.y, run[2] = x.z, run[3] = x.w;
   }

@@ -1246,6 +1246,14 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
                 }
           }
         }
+        if (x.len > 0 && !keeps_state(ld)) {
+#pragma unroll
+          for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+            for (int cg = 0; cg < K::kCg; ++cg)
+#pragma unroll
+              for (int y = 0; y < 16; ++y) S[hh][cg][y] = 0;
+        }
         F2 f[8];
         for (int c = 0; c < x.len; c += kC, ++cc) {
           const int n = min(kC, x.len - c);

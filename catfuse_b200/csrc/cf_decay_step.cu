@@ -44,6 +44,7 @@ __global__ void __launch_bounds__(kStepThreads) decay_step_kernel(const __grid_c
   __shared__ float s_k[kStepMaxDim];
   __shared__ float s_q[kStepMaxDim];
   __shared__ float2 s_decay;
+  __shared__ bool s_keeps;
   __shared__ __align__(16) float s_o[kStepThreads / 32][kStepCols];
   const int slice = blockIdx.x % a.n_slices;
   const int64_t bh = blockIdx.x / a.n_slices;
@@ -78,9 +79,17 @@ __global__ void __launch_bounds__(kStepThreads) decay_step_kernel(const __grid_c
     const T* pv = static_cast<const T*>(a.v) + b * a.v_st + h * a.v_sh + c;
     v = make_float4(to_f(pv[0]), to_f(pv[1]), to_f(pv[2]), to_f(pv[3]));
   }
-  if (tid == 0) s_decay = decay_hi_lo(a.log_decay[h]);
+  if (tid == 0) {
+    const float ld = a.log_decay[h];
+    s_decay = decay_hi_lo(ld);
+    s_keeps = keeps_state(ld);
+  }
   __syncthreads();
   const float2 decay = s_decay;
+  if (!s_keeps) {
+#pragma unroll
+    for (int i = 0; i < kStepRows; ++i) s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
 #pragma unroll
   for (int i = 0; i < kStepRows; ++i) {
     const int r = i * kStepRowGroups + rg;

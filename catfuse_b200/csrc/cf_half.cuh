@@ -28,4 +28,8 @@ __device__ __forceinline__ float2 decay_hi_lo(float log_decay) {
   return make_float2(hi, isfinite(hi) ? (float)(l - (double)hi) : 0.f);
 }
 
+// Whether a head's state outlives a token.  What enters one that keeps nothing
+// (log_decay = -inf) is not looked at: it may be anything, and 0 * inf is no zero.
+__device__ __forceinline__ bool keeps_state(float log_decay) { return log_decay != -INFINITY; }
+
 }  // namespace cf

@@ -85,3 +85,43 @@ def test_silent_tail_under_steep_decays(dev, dtype, n, dims):
     ops.decay_attention(q[None], k[None], v[None], ld, s_out=s)
     _, S, _, aS = chunked(q, k, v, ld)
     check_state(s[0], S, aS)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("length", [1, 70, 5000])
+def test_a_head_that_keeps_nothing_drops_a_non_finite_state(dev, dtype, odd, length):
+    from catfuse_b200 import ops
+    h, d = 2, 64
+    g = torch.Generator(device=dev).manual_seed(4)
+    pad = 1 if odd else 0  # rows off 16 bytes
+    q, k, v = [torch.randn(2 * length, h, d + pad, generator=g, device=dev).to(dtype)[..., pad:] for _ in range(3)]
+    ld = torch.tensor([float("-inf"), -0.1], device=dev)
+    s0 = torch.randn(3, h, d, d, generator=g, device=dev)
+    bad = s0.clone()
+    for r, x in enumerate((float("nan"), float("inf"), float("nan"))):
+        bad[r, 0] = x
+    cu = torch.tensor([0, length, length, 2 * length], dtype=torch.int32, device=dev)
+    want_s, got_s = s0.clone(), bad.clone()
+    want = ops.decay_attention(q, k, v, ld, s_in=want_s, s_out=want_s, cu_seqlens=cu)
+    got = ops.decay_attention(q, k, v, ld, s_in=got_s, s_out=got_s, cu_seqlens=cu)
+    assert torch.equal(got, want) and torch.equal(got_s[::2], want_s[::2])
+    assert torch.isinf(got_s[1, 0]).all()  # no tokens: the state as it was
+    dense = [t.unflatten(0, (2, length)) for t in (q, k, v)]
+    want_s, got_s = s0[:2].clone(), bad[:2].clone()
+    want = ops.decay_attention(*dense, ld, s_in=want_s, s_out=want_s)
+    got = ops.decay_attention(*dense, ld, s_in=got_s, s_out=got_s)
+    assert torch.equal(got, want) and torch.equal(got_s, want_s)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_step_of_a_head_that_keeps_nothing(dev, dtype):
+    from catfuse_b200 import ops
+    q, k, v = [torch.randn(3, 2, 64, device=dev).to(dtype) for _ in range(3)]
+    ld = torch.tensor([float("-inf"), -0.1], device=dev)
+    s0 = torch.randn(3, 2, 64, 64, device=dev)
+    bad = s0.clone()
+    bad[0, 0], bad[1, 0], bad[2, 0] = float("nan"), float("inf"), -float("inf")
+    want = ops.decay_attention_step(q, k, v, ld, s0)
+    got = ops.decay_attention_step(q, k, v, ld, bad)
+    assert torch.equal(got, want) and torch.equal(bad, s0)
