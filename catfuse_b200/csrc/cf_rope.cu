@@ -53,6 +53,7 @@ struct RopeArgs {
   const float* k_weight;
   int64_t N;
   int Hq, Hk, D, rot, half_pairs, norm;  // half_pairs: pairs are (p, p + rot/2)
+  int partial;      // some channels pass through
   int lpr, splits;  // lanes of a row, warps of a token
   float eps;
   uint8_t axis[kRopeMaxDim / 2];
@@ -274,8 +275,13 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
             unpack2(r, u, v);
             r = pack2(v, u);
           }
-          unpack2(mul2(fma2(p, c1[j][i], mul2(x[j][i], c0[j][i])), inv2), e[2 * i], e[2 * i + 1]);
-          unpack2(mul2(fma2(r, c3[j][i], mul2(y[j][i], c2[j][i])), inv2), f[2 * i], f[2 * i + 1]);
+          F2 u = mul2(x[j][i], c0[j][i]), v = mul2(y[j][i], c2[j][i]);
+          if (!a.partial || sub + j * lpr < RU) {  // else no partner: 0 * inf must not appear
+            u = fma2(p, c1[j][i], u);
+            v = fma2(r, c3[j][i], v);
+          }
+          unpack2(mul2(u, inv2), e[2 * i], e[2 * i + 1]);
+          unpack2(mul2(v, inv2), f[2 * i], f[2 * i + 1]);
         }
         if (put && sub + j * lpr < NU) {
           store_vec<T, V>(dst + ca[j], e);
@@ -389,7 +395,7 @@ extern "C" int cf_qk_norm_rope(const void* q, const void* k, void* q_out, void* 
   a.pos = positions; a.pos_stride = pos_stride; a.pos64 = pos_bits == 64;
   a.inv_freq = inv_freq; a.q_weight = q_weight; a.k_weight = k_weight;
   a.N = N; a.Hq = (int)Hq; a.Hk = (int)Hk; a.D = (int)D; a.rot = (int)rot;
-  a.half_pairs = pairing == CF_PAIR_HALF; a.norm = norm; a.eps = eps;
+  a.half_pairs = pairing == CF_PAIR_HALF; a.partial = rot < D; a.norm = norm; a.eps = eps;
   if (N > 0x7FFFFFFF) return fail(CF_ERR_UNSUPPORTED, "too many tokens");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return fmt == CF_FMT_F16 ? launch_rope_v<__half>(a, V, s) : launch_rope_v<__nv_bfloat16>(a, V, s);
