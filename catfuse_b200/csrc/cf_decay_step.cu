@@ -44,7 +44,6 @@ __global__ void __launch_bounds__(kStepThreads) decay_step_kernel(const __grid_c
   __shared__ float s_k[kStepMaxDim];
   __shared__ float s_q[kStepMaxDim];
   __shared__ float2 s_decay;
-  __shared__ bool s_keeps;
   __shared__ __align__(16) float s_o[kStepThreads / 32][kStepCols];
   const int slice = blockIdx.x % a.n_slices;
   const int64_t bh = blockIdx.x / a.n_slices;
@@ -81,24 +80,23 @@ __global__ void __launch_bounds__(kStepThreads) decay_step_kernel(const __grid_c
   }
   if (tid == 0) {
     const float ld = a.log_decay[h];
-    s_decay = decay_hi_lo(ld);
-    s_keeps = keeps_state(ld);
+    s_decay = keeps_state(ld) ? decay_hi_lo(ld) : make_float2(-1.f, 0.f);
   }
   __syncthreads();
   const float2 decay = s_decay;
-  if (!s_keeps) {
-#pragma unroll
-    for (int i = 0; i < kStepRows; ++i) s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
+  // -1: nothing is kept, and what was loaded may be anything; masked to zeros
+  const uint32_t kept = decay.x == -1.f ? 0u : ~0u;
+  auto held = [&](float x) { return __uint_as_float(__float_as_uint(x) & kept); };
 #pragma unroll
   for (int i = 0; i < kStepRows; ++i) {
     const int r = i * kStepRowGroups + rg;
     if (on && r < a.Dk) {
       const float k = s_k[r];
-      s[i].x = fmaf(decay.x, s[i].x, fmaf(decay.y, s[i].x, k * v.x));
-      s[i].y = fmaf(decay.x, s[i].y, fmaf(decay.y, s[i].y, k * v.y));
-      s[i].z = fmaf(decay.x, s[i].z, fmaf(decay.y, s[i].z, k * v.z));
-      s[i].w = fmaf(decay.x, s[i].w, fmaf(decay.y, s[i].w, k * v.w));
+      const float4 e = make_float4(held(s[i].x), held(s[i].y), held(s[i].z), held(s[i].w));
+      s[i].x = fmaf(decay.x, e.x, fmaf(decay.y, e.x, k * v.x));
+      s[i].y = fmaf(decay.x, e.y, fmaf(decay.y, e.y, k * v.y));
+      s[i].z = fmaf(decay.x, e.z, fmaf(decay.y, e.z, k * v.z));
+      s[i].w = fmaf(decay.x, e.w, fmaf(decay.y, e.w, k * v.w));
       __stcs(reinterpret_cast<float4*>(a.s_out + base + (int64_t)r * a.Dv), s[i]);
     }
   }
