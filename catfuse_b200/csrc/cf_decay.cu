@@ -132,11 +132,12 @@ __global__ void __launch_bounds__(kThreads) decay_recurrent_kernel(const __grid_
 // --------------------------------------------------------------------------
 
 // The segments of packed sequences, in order: every sequence has one at least.
-// Entries that are left over have seq = -1.
+// Entries that are left over have seq = -1.  Sums are 64 bits wide: overlapping
+// boundaries can ask for far more segments than there are entries.
 __global__ void __launch_bounds__(1024) decay_segments_kernel(const int32_t* cu, int S, int64_t N, int64_t seg_len,
                                                               Seg* segs, int32_t* first, int n_segs) {
-  __shared__ int s_sum[32];
-  __shared__ int s_base;
+  __shared__ int64_t s_sum[32];
+  __shared__ int64_t s_base;
   griddep_wait();
   griddep_launch_dependents();
   if (threadIdx.x == 0) s_base = 0;
@@ -151,25 +152,25 @@ __global__ void __launch_bounds__(1024) decay_segments_kernel(const int32_t* cu,
       t1 = min(max((int64_t)cu[s + 1], t0), N);
       n = t1 > t0 ? (int)((t1 - t0 + seg_len - 1) / seg_len) : 1;
     }
-    int x = n;
+    int64_t x = n;
     for (int m = 1; m < 32; m <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, m);
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
       if (lane >= m) x += y;
     }
     if (lane == 31) s_sum[warp] = x;
     __syncthreads();
     if (warp == 0) {
-      int y = s_sum[lane];
+      int64_t y = s_sum[lane];
       for (int m = 1; m < 32; m <<= 1) {
-        const int z = __shfl_up_sync(0xffffffffu, y, m);
+        const int64_t z = __shfl_up_sync(0xffffffffu, y, m);
         if (lane >= m) y += z;
       }
       s_sum[lane] = y;
     }
     __syncthreads();
-    int at = s_base + x - n + (warp ? s_sum[warp - 1] : 0);
+    int64_t at = s_base + x - n + (warp ? s_sum[warp - 1] : 0);
     if (s < S) {
-      first[s] = min(at, n_segs);  // more only if the sequences overlap
+      first[s] = (int32_t)min(at, (int64_t)n_segs);  // more only if the sequences overlap
       for (int i = 0; i < n && at < n_segs; ++i, ++at) {
         const int64_t b = t0 + i * seg_len;
         segs[at] = Seg{(int32_t)b, (int32_t)min(b + seg_len, t1), s, i == n - 1};
@@ -179,8 +180,8 @@ __global__ void __launch_bounds__(1024) decay_segments_kernel(const int32_t* cu,
     if (threadIdx.x == 0) s_base += s_sum[31];
     __syncthreads();
   }
-  for (int i = s_base + threadIdx.x; i < n_segs; i += 1024) segs[i] = Seg{0, 0, -1, 0};
-  if (threadIdx.x == 0) first[S] = min(s_base, n_segs);
+  for (int64_t i = s_base + threadIdx.x; i < n_segs; i += 1024) segs[i] = Seg{0, 0, -1, 0};
+  if (threadIdx.x == 0) first[S] = (int32_t)min(s_base, (int64_t)n_segs);
 }
 
 // A segment's own state L_r becomes the state that enters it:
