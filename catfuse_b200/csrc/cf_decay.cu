@@ -131,57 +131,62 @@ __global__ void __launch_bounds__(kThreads) decay_recurrent_kernel(const __grid_
 // segments
 // --------------------------------------------------------------------------
 
-// The segments of packed sequences, in order: every sequence has one at least.
+// Sum over the block's threads before and including this one; total over all of them.
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* s_sum, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int m = 1; m < 32; m <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
+    if (lane >= m) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) s_sum[warp] = x;
+  __syncthreads();
+  total = 0;
+  int64_t before = 0;
+  for (int w = 0; w < 32; ++w) {
+    if (w == warp) before = total;
+    total += s_sum[w];
+  }
+  return x + before;
+}
+
+// The segments of packed sequences, in order: every sequence has one at least, and
+// those with more have a row of seg_states for each (first: the first of them).
 // Entries that are left over have seq = -1.  Sums are 64 bits wide: overlapping
-// boundaries can ask for far more segments than there are entries.
+// boundaries can ask for far more segments and rows than there are, and get no more.
 __global__ void __launch_bounds__(1024) decay_segments_kernel(const int32_t* cu, int S, int64_t N, int64_t seg_len,
-                                                              Seg* segs, int32_t* first, int n_segs) {
+                                                              Seg* segs, int32_t* first, int64_t n_segs,
+                                                              int64_t n_rows) {
   __shared__ int64_t s_sum[32];
-  __shared__ int64_t s_base;
   griddep_wait();
   griddep_launch_dependents();
-  if (threadIdx.x == 0) s_base = 0;
-  __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t base = 0, row_base = 0;
   for (int s0 = 0; s0 < S; s0 += 1024) {
     const int s = s0 + threadIdx.x;
-    int64_t t0 = 0, t1 = 0;
-    int n = 0;
+    int64_t t0 = 0, t1 = 0, n = 0;
     if (s < S) {
       t0 = min(max((int64_t)cu[s], (int64_t)0), N);
       t1 = min(max((int64_t)cu[s + 1], t0), N);
-      n = t1 > t0 ? (int)((t1 - t0 + seg_len - 1) / seg_len) : 1;
+      n = t1 > t0 ? (t1 - t0 + seg_len - 1) / seg_len : 1;
     }
-    int64_t x = n;
-    for (int m = 1; m < 32; m <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
-      if (lane >= m) x += y;
-    }
-    if (lane == 31) s_sum[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-      int64_t y = s_sum[lane];
-      for (int m = 1; m < 32; m <<= 1) {
-        const int64_t z = __shfl_up_sync(0xffffffffu, y, m);
-        if (lane >= m) y += z;
-      }
-      s_sum[lane] = y;
-    }
-    __syncthreads();
-    int64_t at = s_base + x - n + (warp ? s_sum[warp - 1] : 0);
+    const int64_t own_rows = n > 1 ? n : 0;
+    int64_t total, rows;
+    int64_t at = base + block_scan(n, s_sum, total) - n;
+    int64_t row = row_base + block_scan(own_rows, s_sum, rows) - own_rows;
     if (s < S) {
-      first[s] = (int32_t)min(at, (int64_t)n_segs);  // more only if the sequences overlap
-      for (int i = 0; i < n && at < n_segs; ++i, ++at) {
+      first[s] = (int32_t)min(row, n_rows);
+      for (int64_t i = 0; i < n && at < n_segs; ++i, ++at, ++row) {
         const int64_t b = t0 + i * seg_len;
-        segs[at] = Seg{(int32_t)b, (int32_t)min(b + seg_len, t1), s, i == n - 1};
+        const bool in = n == 1 || row < n_rows;
+        segs[at] = Seg{(int32_t)b, (int32_t)min(b + seg_len, t1), in ? s : -1,
+                       (n == 1 ? 0 : (int32_t)min(row, n_rows) * 2) + (i == n - 1)};
       }
     }
-    __syncthreads();
-    if (threadIdx.x == 0) s_base += s_sum[31];
-    __syncthreads();
+    base += total;
+    row_base += rows;
   }
-  for (int64_t i = s_base + threadIdx.x; i < n_segs; i += 1024) segs[i] = Seg{0, 0, -1, 0};
-  if (threadIdx.x == 0) first[S] = (int32_t)min(s_base, (int64_t)n_segs);
+  for (int64_t i = base + threadIdx.x; i < n_segs; i += 1024) segs[i] = Seg{0, 0, -1, 0};
+  if (threadIdx.x == 0) first[S] = (int32_t)min(row_base, n_rows);
 }
 
 // A segment's own state L_r becomes the state that enters it:
@@ -248,7 +253,7 @@ int sm_count() {
 }
 
 struct Plan {
-  int64_t seg_len, n_segs, state_bytes, bytes;
+  int64_t seg_len, n_segs, n_rows, state_bytes, bytes;  // n_rows: states of cut sequences' segments
   int n_seg;  // segments of each sequence (dense)
   bool split;
 };
@@ -280,7 +285,7 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
           p.seg_len = len * kC;
         }
       }
-      p.n_segs = S * p.n_seg;
+      p.n_segs = p.n_rows = S * p.n_seg;
       p.split = p.n_seg > 1;
     } else {
       // Lengths are on the device.  The shorter the segments, the more evenly
@@ -292,12 +297,14 @@ Plan make_plan(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk, int64_t
       if (N > len * kC) {
         p.seg_len = len * kC;
         p.n_segs = S + N / p.seg_len;
+        // a cut sequence has more than seg_len tokens, and one segment that is not full
+        p.n_rows = N / p.seg_len + (S < N / p.seg_len ? S : N / p.seg_len);
         p.split = true;
       }
     }
   }
   if (p.split) {
-    p.state_bytes = p.n_segs * Hk * Dk * Dv * 4;
+    p.state_bytes = p.n_rows * Hk * Dk * Dv * 4;
     p.bytes = p.state_bytes + (packed ? p.n_segs * (int64_t)sizeof(Seg) + (S + 1) * 4 : 0);
     p.bytes = (p.bytes + 15) / 16 * 16;
   }
@@ -444,7 +451,7 @@ extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, v
       first = reinterpret_cast<int32_t*>(segs + p.n_segs);
       a.segs = segs;
       if (int rc = launch_after(decay_segments_kernel, dim3(1), 1024, st, "decay segments launch", cu_seqlens,
-                                (int)S, N, p.seg_len, segs, first, (int)p.n_segs))
+                                (int)S, N, p.seg_len, segs, first, p.n_segs, p.n_rows))
         return rc;
     }
     a.n_units = (uint32_t)((cu_seqlens ? p.n_segs : S * (p.n_seg - 1)) * Hk);

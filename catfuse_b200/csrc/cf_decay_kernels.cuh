@@ -72,7 +72,7 @@ enum : int32_t {
 };
 
 struct Seg {  // one segment of one packed sequence
-  int32_t t0, t1, seq, last;
+  int32_t t0, t1, seq, row_last;  // its row of seg_states (if the sequence is cut) * 2 + whether it is the last
 };
 
 struct DecayArgs {
@@ -86,7 +86,7 @@ struct DecayArgs {
   const int32_t* slots;
   const int32_t* cu;
   const Seg* segs;    // packed sequences in segments, else NULL
-  float* seg_states;  // [segment][Hk][Dk][Dv]: a segment's own state, then the one that enters it
+  float* seg_states;  // [row][Hk][Dk][Dv]: a segment's own state, then the one that enters it
   int64_t n_slots, L, N, seg_len;  // seg_len: tokens of a segment, a multiple of 64 (or >= every length)
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;
   uint32_t n_units;   // segments x heads, below 2^31
@@ -481,7 +481,8 @@ __device__ __forceinline__ bool get_unit(const DecayArgs& a, uint32_t u, Unit& x
     x.seq = s.seq;
     x.t0 = s.t0;
     x.len = s.t1 - s.t0;
-    last = s.last != 0;
+    seg = s.row_last >> 1;
+    last = s.row_last & 1;
     first = sg == 0 || a.segs[sg - 1].seq != s.seq;
   } else if (a.cu) {
     x.seq = (int)sg;
