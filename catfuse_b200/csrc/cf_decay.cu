@@ -405,6 +405,8 @@ extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, v
   for (const void* p : {(const void*)s_in, (const void*)s_out, (const void*)workspace})
     if (reinterpret_cast<uintptr_t>(p) & 15)
       return fail(CF_ERR_UNSUPPORTED, "states and workspace must be 16-byte aligned");
+  if (!rows_apart(N, o_st, Hq, o_sh, Dv))
+    return fail(CF_ERR_INVALID_ARG, "rows of out overlap");
   if (int rc = require_sm100()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   DecayArgs a{};

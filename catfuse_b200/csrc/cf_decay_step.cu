@@ -159,6 +159,8 @@ extern "C" int cf_decay_attention_step(const void* q, const void* k, const void*
   const int64_t slices = (Dv + kStepCols - 1) / kStepCols;
   if (Hq > 65536 || B > 0x7FFFFFFF / (Hk * slices))
     return fail(CF_ERR_UNSUPPORTED, "too many sequences or heads");
+  if (!rows_apart(B, o_st, Hq, o_sh, Dv))
+    return fail(CF_ERR_INVALID_ARG, "rows of out overlap");
   if (int rc = require_sm100()) return rc;
   StepArgs a{q, k, v, out, log_decay, s_in, s_out, slots, n_slots, q_st, q_sh, k_st, k_sh,
              v_st, v_sh, o_st, o_sh, (int)Hq, (int)Hk, (int)Dk, (int)Dv, (int)slices, scale};

@@ -19,6 +19,16 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
+// Whether the rows of an output (d elements; n of them st apart, of each h heads sh
+// apart) share no element: where they do, the value left would be either writer's.
+inline bool rows_apart(int64_t n, int64_t st, int64_t h, int64_t sh, int64_t d) {
+  st = st < 0 ? -st : st;
+  sh = sh < 0 ? -sh : sh;
+  if (n <= 1) return n == 0 || h <= 1 || sh >= d;
+  if (h <= 1) return st >= d;
+  return st < sh ? st >= d && (n - 1) <= (sh - d) / st : sh >= d && (h - 1) <= (st - d) / sh;
+}
+
 // A head's decay l = exp(log_decay) as hi + lo, so that l s is
 // fma(hi, s, lo s): with l rounded to fp32 alone, a state that forgets slowly
 // would drift by 2^-25 of itself at every token.

@@ -387,6 +387,8 @@ extern "C" int cf_qk_norm_rope(const void* q, const void* k, void* q_out, void* 
   for (const void* p : ptrs)
     if (reinterpret_cast<uintptr_t>(p) & 1)
       return fail(CF_ERR_UNSUPPORTED, "q, k and their outputs must be aligned to their type");
+  if (!rows_apart(N, qo_st, Hq, qo_sh, D) || !rows_apart(N, ko_st, Hk, ko_sh, D))
+    return fail(CF_ERR_INVALID_ARG, "rows of an output overlap");
   if (int rc = require_sm100()) return rc;
 
   a.q = q; a.k = k; a.q_out = q_out; a.k_out = k_out;
