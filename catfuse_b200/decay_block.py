@@ -30,7 +30,8 @@ class DecayAttentionLIF(nn.Module):
     ``heads`` query heads of ``head_dim`` share ``kv_heads`` states.  ``sections``
     gives the rotated pairs of each position axis (one axis: text; three: time,
     height and width of a patch stream); positions are [B, L] or [axes, B, L].
-    The decays run from e^-1 to e^-1/512 over the states."""
+    The decays run from e^-1 to e^-1/512 over the states.  ``dtype`` (fp16 or bf16, also
+    by ``.half()`` or ``.to(dtype)``) is that of the projections and what lies between."""
 
     def __init__(self, dim: int, heads: int, kv_heads: Optional[int] = None,
                  head_dim: Optional[int] = None, sections=None, axis_order: str = "blocks",
@@ -48,6 +49,17 @@ class DecayAttentionLIF(nn.Module):
         self.q_weight = nn.Parameter(torch.ones(self.head_dim))
         self.k_weight = nn.Parameter(torch.ones(self.head_dim))
         self.state, self.membrane = StateBuffer(), StateBuffer()
+
+    def _apply(self, fn, recurse=True):
+        # what the operators take in fp32 stays in fp32 under .half() and .to(dtype)
+        names = ("inv_freq", "log_decay", "q_weight", "k_weight")
+        kept = {n: getattr(self, n).data for n in names}
+        super()._apply(fn, recurse)
+        for n in names:
+            t = getattr(self, n)
+            if t.dtype != torch.float32:
+                t.data = kept[n].to(t.device)
+        return self
 
     def reset(self) -> None:
         self.state.reset()

@@ -1,0 +1,23 @@
+"""DecayAttentionLIF without a device: what its conversions and refusals leave."""
+import pytest
+import torch
+
+from catfuse_b200.decay_block import DecayAttentionLIF
+
+FP32 = ("inv_freq", "log_decay", "q_weight", "k_weight")
+
+
+@pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.float16),
+                                     lambda m: torch.nn.Sequential(m).to(torch.bfloat16)[0],
+                                     lambda m: m.half().bfloat16()])
+def test_conversions_keep_the_fp32_parts(convert):
+    m = DecayAttentionLIF(64, heads=4, kv_heads=2)
+    with torch.no_grad():
+        m.q_weight.uniform_(0.5, 1.5)
+    before = {n: getattr(m, n).detach().clone() for n in FP32}
+    convert(m)
+    assert m.qkv.weight.dtype == m.proj.weight.dtype != torch.float32
+    for n in FP32:
+        t = getattr(m, n)
+        assert t.dtype == torch.float32 and torch.equal(t, before[n])
+    assert {"q_weight", "k_weight"} <= dict(m.named_parameters()).keys()
