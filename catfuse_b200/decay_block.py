@@ -7,7 +7,8 @@ for streams: one fused q/k/v projection, a norm and rotation of queries and keys
 token (``ops.decay_attention`` for prompts, ``ops.decay_attention_step`` for single
 tokens), an output projection, and a LIF neuron whose time axis is the token axis
 (``ops.lif_fwd``).  The attention states and the membrane are carried from call to
-call until ``reset()``, so a prompt may come whole, in pieces, or token by token.
+call until ``reset()``, so a prompt may come whole, in pieces, or token by token;
+another number of streams needs a ``reset()``.
 
     python -m catfuse_b200.decay_block      # a prompt, then tokens, timed
 """
@@ -65,6 +66,14 @@ class DecayAttentionLIF(nn.Module):
         self.state.reset()
         self.membrane.reset()
 
+    def _check_streams(self, x) -> int:
+        """The batch, which must be that of the carried states."""
+        B, held = x.shape[0], self.state.tensor
+        if held is not None and (held.shape[0] != B or held.device != x.device):
+            raise ValueError(f"the block carries the states of {held.shape[0]} streams on {held.device}, got "
+                             f"{B} on {x.device}: call reset() first")
+        return B
+
     def _project(self, x, positions):
         h, hk, d = self.heads, self.kv_heads, self.head_dim
         qkv = self.qkv(x.to(self.qkv.weight.dtype))
@@ -83,7 +92,7 @@ class DecayAttentionLIF(nn.Module):
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-        B = x.shape[0]
+        B = self._check_streams(x)
         q, k, v = self._project(x, positions)
         s = self.state.get((B, self.kv_heads, self.head_dim, self.head_dim), x.device)
         y = ops.decay_attention(q, k, v, self.log_decay, s_in=s, s_out=s)
@@ -91,7 +100,7 @@ class DecayAttentionLIF(nn.Module):
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-        B = x.shape[0]
+        B = self._check_streams(x)
         q, k, v = self._project(x, positions)
         s = self.state.get((B, self.kv_heads, self.head_dim, self.head_dim), x.device)
         y = ops.decay_attention_step(q, k, v, self.log_decay, s)

@@ -21,3 +21,16 @@ def test_conversions_keep_the_fp32_parts(convert):
         t = getattr(m, n)
         assert t.dtype == torch.float32 and torch.equal(t, before[n])
     assert {"q_weight", "k_weight"} <= dict(m.named_parameters()).keys()
+
+
+@pytest.mark.parametrize("tokens", [None, 5])
+def test_another_batch_is_refused_and_the_states_stay(tokens):
+    m = DecayAttentionLIF(64, heads=4, kv_heads=2)
+    state, membrane = torch.randn(2, 2, 16, 16), torch.randn(2, 64)
+    m.state.set(state.clone())
+    m.membrane.set(membrane.clone())
+    x = torch.randn(3, 64) if tokens is None else torch.randn(3, tokens, 64)
+    pos = torch.zeros(x.shape[:-1], dtype=torch.int32)
+    with pytest.raises(ValueError, match="reset"):
+        (m.step if tokens is None else m)(x, pos)
+    assert torch.equal(m.state.tensor, state) and torch.equal(m.membrane.tensor, membrane)
