@@ -93,6 +93,8 @@ class DecayAttentionLIF(nn.Module):
     @torch.no_grad()
     def forward(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         B = self._check_streams(x)
+        if x.shape[1] == 0:  # nothing to attend to: states and membrane stay as they are
+            return x.new_zeros(x.shape, dtype=torch.float32)
         q, k, v = self._project(x, positions)
         s = self.state.get((B, self.kv_heads, self.head_dim, self.head_dim), x.device)
         y = ops.decay_attention(q, k, v, self.log_decay, s_in=s, s_out=s)

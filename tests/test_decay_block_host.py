@@ -34,3 +34,18 @@ def test_another_batch_is_refused_and_the_states_stay(tokens):
     with pytest.raises(ValueError, match="reset"):
         (m.step if tokens is None else m)(x, pos)
     assert torch.equal(m.state.tensor, state) and torch.equal(m.membrane.tensor, membrane)
+
+
+@pytest.mark.parametrize("carried", [False, True])
+def test_a_prompt_without_tokens_changes_nothing(carried):
+    m = DecayAttentionLIF(64, heads=4, kv_heads=2)
+    state, membrane = torch.randn(2, 2, 16, 16), torch.randn(2, 64)
+    if carried:
+        m.state.set(state.clone())
+        m.membrane.set(membrane.clone())
+    out = m(torch.zeros(2, 0, 64), torch.zeros(2, 0, dtype=torch.int32))
+    assert out.shape == (2, 0, 64) and out.dtype == torch.float32
+    if carried:
+        assert torch.equal(m.state.tensor, state) and torch.equal(m.membrane.tensor, membrane)
+    else:
+        assert m.state.tensor is None and m.membrane.tensor is None
