@@ -1379,7 +1379,7 @@ __global__ void __launch_bounds__(Cfg<T, DK, DV, OUT>::kThreads, Cfg<T, DK, DV, 
       }
     }
 
-    if (!ok) give_up(TM && wg == K::kV ? ERR_SITE_DECAY_V : ERR_SITE_DECAY_STATE, w);
+    if (!ok) give_up(K::kV != K::kS && wg == K::kV ? ERR_SITE_DECAY_V : ERR_SITE_DECAY_STATE, w);
   }
 
   tc_fence_before();
