@@ -131,59 +131,64 @@ __global__ void __launch_bounds__(kThreads) decay_recurrent_kernel(const __grid_
 // segments
 // --------------------------------------------------------------------------
 
-// Sum over the block's threads before and including this one; total over all of them.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* s_sum, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+template <typename I>
+__device__ __forceinline__ I warp_scan(I x) {  // over the lanes up to this one
   for (int m = 1; m < 32; m <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
-    if (lane >= m) x += y;
+    const I y = __shfl_up_sync(0xffffffffu, x, m);
+    if ((threadIdx.x & 31) >= m) x += y;
   }
-  __syncthreads();
-  if (lane == 31) s_sum[warp] = x;
-  __syncthreads();
-  total = 0;
-  int64_t before = 0;
-  for (int w = 0; w < 32; ++w) {
-    if (w == warp) before = total;
-    total += s_sum[w];
-  }
-  return x + before;
+  return x;
 }
 
 // The segments of packed sequences, in order: every sequence has one at least, and
 // those with more have a row of seg_states for each (first: the first of them).
-// Entries that are left over have seq = -1.  Sums are 64 bits wide: overlapping
-// boundaries can ask for far more segments and rows than there are, and get no more.
+// Entries that are left over have seq = -1.  Sums over more than a warp's sequences (2^23
+// segments each at most) are 64 bits wide: overlapping boundaries can ask for far more
+// segments and rows than there are, and get no more.
 __global__ void __launch_bounds__(1024) decay_segments_kernel(const int32_t* cu, int S, int64_t N, int64_t seg_len,
                                                               Seg* segs, int32_t* first, int64_t n_segs,
                                                               int64_t n_rows) {
-  __shared__ int64_t s_sum[32];
+  __shared__ int32_t s_n[32], s_rows[32];
   griddep_wait();
   griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t base = 0, row_base = 0;
   for (int s0 = 0; s0 < S; s0 += 1024) {
     const int s = s0 + threadIdx.x;
-    int64_t t0 = 0, t1 = 0, n = 0;
+    int64_t t0 = 0, t1 = 0;
+    int32_t n = 0;
     if (s < S) {
       t0 = min(max((int64_t)cu[s], (int64_t)0), N);
       t1 = min(max((int64_t)cu[s + 1], t0), N);
-      n = t1 > t0 ? (t1 - t0 + seg_len - 1) / seg_len : 1;
+      n = t1 > t0 ? (int32_t)((t1 - t0 + seg_len - 1) / seg_len) : 1;
     }
-    const int64_t own_rows = n > 1 ? n : 0;
-    int64_t total, rows;
-    int64_t at = base + block_scan(n, s_sum, total) - n;
-    int64_t row = row_base + block_scan(own_rows, s_sum, rows) - own_rows;
+    const int32_t own_rows = n > 1 ? n : 0;
+    const int32_t n_to = warp_scan(n), rows_to = warp_scan(own_rows);
+    if (lane == 31) {
+      s_n[warp] = n_to;
+      s_rows[warp] = rows_to;
+    }
+    __syncthreads();
+    const int64_t n_all = warp_scan((int64_t)s_n[lane]), rows_all = warp_scan((int64_t)s_rows[lane]);
+    int64_t at = base + n_to - n, row = row_base + rows_to - own_rows;
+    const int64_t n_before = __shfl_sync(0xffffffffu, n_all, (warp + 31) & 31);
+    const int64_t rows_before = __shfl_sync(0xffffffffu, rows_all, (warp + 31) & 31);
+    if (warp > 0) {
+      at += n_before;
+      row += rows_before;
+    }
     if (s < S) {
       first[s] = (int32_t)min(row, n_rows);
-      for (int64_t i = 0; i < n && at < n_segs; ++i, ++at, ++row) {
+      for (int i = 0; i < n && at < n_segs; ++i, ++at, ++row) {
         const int64_t b = t0 + i * seg_len;
         const bool in = n == 1 || row < n_rows;
         segs[at] = Seg{(int32_t)b, (int32_t)min(b + seg_len, t1), in ? s : -1,
                        (n == 1 ? 0 : (int32_t)min(row, n_rows) * 2) + (i == n - 1)};
       }
     }
-    base += total;
-    row_base += rows;
+    base += __shfl_sync(0xffffffffu, n_all, 31);
+    row_base += __shfl_sync(0xffffffffu, rows_all, 31);
+    __syncthreads();
   }
   for (int64_t i = base + threadIdx.x; i < n_segs; i += 1024) segs[i] = Seg{0, 0, -1, 0};
   if (threadIdx.x == 0) first[S] = (int32_t)min(row_base, n_rows);
