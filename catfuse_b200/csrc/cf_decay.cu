@@ -412,6 +412,10 @@ extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, v
       return fail(CF_ERR_UNSUPPORTED, "states and workspace must be 16-byte aligned");
   if (!rows_apart(N, o_st, Hq, o_sh, Dv))
     return fail(CF_ERR_INVALID_ARG, "rows of out overlap");
+  const bool recurrence = N == 0 || !tma_rows(q, N, Hq, q_st, q_sh) || !tma_rows(k, N, Hk, k_st, k_sh) ||
+                          !tma_rows(v, N, Hk, v_st, v_sh);
+  if (N && recurrence && Dv > kCols && (out == q || out == k))  // other CTAs of a head read them while one writes
+    return fail(CF_ERR_INVALID_ARG, "out must not be q or k where rows are off 16 bytes");
   if (int rc = require_sm100()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   DecayArgs a{};
@@ -421,8 +425,7 @@ extern "C" int cf_decay_attention(const void* q, const void* k, const void* v, v
   a.o_st = o_st; a.o_sh = o_sh; a.Hq = (int)Hq; a.Hk = (int)Hk; a.Dk = (int)Dk; a.Dv = (int)Dv;
   a.S = (int)S; a.scale = scale; a.n_seg = 1;
 
-  if (N == 0 || !tma_rows(q, N, Hq, q_st, q_sh) || !tma_rows(k, N, Hk, k_st, k_sh) ||
-      !tma_rows(v, N, Hk, v_st, v_sh)) {
+  if (recurrence) {
     const int slices = (int)((Dv + kCols - 1) / kCols);
     const unsigned grid = (unsigned)(S * Hk * slices);
     if (fmt == CF_FMT_F16) decay_recurrent_kernel<__half><<<grid, kThreads, 0, st>>>(a, slices);

@@ -159,6 +159,8 @@ extern "C" int cf_decay_attention_step(const void* q, const void* k, const void*
   const int64_t slices = (Dv + kStepCols - 1) / kStepCols;
   if (Hq > 65536 || B > 0x7FFFFFFF / (Hk * slices))
     return fail(CF_ERR_UNSUPPORTED, "too many sequences or heads");
+  if (slices > 1 && (out == q || out == k))  // other CTAs of a head read them while one writes
+    return fail(CF_ERR_INVALID_ARG, "out must not be q or k");
   if (!rows_apart(B, o_st, Hq, o_sh, Dv))
     return fail(CF_ERR_INVALID_ARG, "rows of out overlap");
   if (int rc = require_sm100()) return rc;

@@ -18,9 +18,9 @@ def test_entry_points_refuse_overlapping_outputs(strides, apart):
     lib = _lib.load()
     good, st = (128, 64), strides
     # addresses are never followed: the last refusal is that there is no device
-    rcs = [lib.cf_decay_attention(16, 16, 16, 16, 1, 16, None, None, None, 0, None, 1, 4, 4, 2, 2, 64, 64,
+    rcs = [lib.cf_decay_attention(16, 16, 16, 64, 1, 16, None, None, None, 0, None, 1, 4, 4, 2, 2, 64, 64,
                                   *good, *good, *good, *st, 1.0, None, 0, None),
-           lib.cf_decay_attention_step(16, 16, 16, 16, 1, 16, 16, 16, None, 4, 4, 2, 2, 64, 64,
+           lib.cf_decay_attention_step(16, 16, 16, 64, 1, 16, 16, 16, None, 4, 4, 2, 2, 64, 64,
                                        *good, *good, *good, *st, 1.0, None)]
     for outs in ((st, good), (good, st)):
         rcs.append(lib.cf_qk_norm_rope(16, 16, 16, 16, 1, 4, 2, 2, 64, *good, *good, *outs[0], *outs[1], 16, 32, 4,
@@ -32,3 +32,16 @@ def test_entry_points_refuse_overlapping_outputs(strides, apart):
         assert rc == _lib.CF_ERR_NO_DEVICE
     for rc in rcs:
         assert rc == (_lib.CF_ERR_NO_DEVICE if apart else _lib.CF_ERR_INVALID_ARG), _lib.last_error()
+
+
+def test_entry_points_refuse_outputs_in_place_of_q_or_k():
+    """The CTAs of a head's 32 columns each share its q and k, so none may write there (rows
+    on 16 bytes of a prompt have one CTA a head, which reads them first)."""
+    from catfuse_b200 import _lib
+    lib = _lib.load()
+    st = (128, 64) * 4
+    for q, k in ((64, 32), (32, 64)):
+        assert lib.cf_decay_attention_step(q, k, 16, 64, 1, 16, 16, 16, None, 4, 4, 2, 2, 64, 64,
+                                           *st, 1.0, None) == _lib.CF_ERR_INVALID_ARG
+        assert lib.cf_decay_attention(q + 2, k + 2, 16, 66, 1, 16, None, None, None, 0, None, 1, 4, 4, 2, 2, 64, 64,
+                                      *st, 1.0, None, 0, None) == _lib.CF_ERR_INVALID_ARG
