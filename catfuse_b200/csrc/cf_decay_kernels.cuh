@@ -31,19 +31,20 @@
 // parts (22 bits).  S and P reach only the 16-bit outputs and are rounded once,
 // which makes the outputs' error 1.42 times that of their own rounding alone.
 // In fp16 every row of V', S and P is scaled by a power of two of its own, so that
-// neither a full state nor a small one leaves the type's range; bf16 has fp32's.  A term of V'
-// below 2^-17 of its row's largest is held to 2^-39 of that.
+// neither a full state nor a small one leaves the type's range; bf16 has fp32's.  What lies
+// far below its row's largest is held to 2^-39 of that: terms of V' below 2^-17, of S and P below
+// 2^-28 of it.
 //
 // Warpgroups: P (QK -> P), O (outputs), S (state), V (V'; in the walk with 64 channels
 // the S warps do it), and one with the TMA and the MMA warp.
 //
-// Measured on one B200 (2048 tokens of 148 sequences x heads, one of each a CTA; HBM floor at
-// 6547 GB/s in brackets): bf16 128 x 128 channels 77 us (50), with four query heads
-// a state 171 us (122), fp16 108 us (50); 296 of 64 x 64 channels, bf16 94 us,
-// fp16 96 us (49).  A chunk takes 3000 cycles of the 2850 that HBM needs with
+// Measured on one B200 (2048 tokens of 148 sequences x heads, one of each a CTA, as graphs back
+// to back; HBM floor at 6547 GB/s in brackets): bf16 128 x 128 channels 77 us (50), with four
+// query heads a state 165 us (122), fp16 105 us (50); 296 of 64 x 64 channels, bf16 90 us,
+// fp16 97 us (49).  A chunk takes 3000 cycles of the 2850 that HBM needs with
 // 128 channels in bf16; the rest of the 77 us is the ends: launch, 64 KB of state in
 // and out, the first chunk through a cold pipeline.  In fp16 the row scales lengthen
-// the S and V roles to 4000 cycles; with 64 channels the S warps' chain V' -> KV -> S
+// the S and V roles by a third; with 64 channels the S warps' chain V' -> KV -> S
 // takes 2700 a chunk and SM, where HBM would need 1430.  The roles wait for
 // instructions and for each other more than for any pipe (tensor pipe 29 %, shared
 // memory 14 %, a scheduler issues in 0.34 of its cycles).

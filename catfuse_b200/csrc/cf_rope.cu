@@ -25,11 +25,12 @@
 // (With weights and rotation applied one after the other and a rounded square root
 // and division, four rows of 128 channels took 390 instructions and the case below 64 us.)
 //
-// Measured: 8192 tokens of 32 + 8 heads of 128 in bf16, 45 us = 3.7 TB/s; 12544 tokens of
+// Measured: 8192 tokens of 32 + 8 heads of 128 in bf16, 46 us = 3.6 TB/s; 12544 tokens of
 // 16 + 16 heads of 80 in fp16 on three axes (4-byte vectors, since half of 60 rotated
-// channels is no multiple of 8 bytes), 52 us = 2.5 TB/s.  A scheduler issues in 0.56 of
-// its cycles with 14 warps an SM (119 registers); capped at 80 registers it spilled
-// and lost more than the occupancy gained.
+// channels is no multiple of 8 bytes), 54 us = 2.4 TB/s.  Bound by its instructions: 21 and 35
+// an element where converting, summing, turning and storing need about 4; a scheduler issues in
+// 0.57 and 0.62 of its cycles with 14 warps an SM (123 registers; capped at 80 it
+// spilled and lost more than the occupancy gained).
 #include "cf_half.cuh"
 
 namespace cf {

@@ -765,7 +765,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     log_decay [Hk] fp32 at most 0.  scale defaults to Dk ** -0.5.  s_in / s_out
     [rows, Hk, Dk, Dv] fp32 carry the state (s_out may be s_in); ``slots`` int32
     names the row of each sequence (outside the rows: start from zeros, store
-    nothing).  Returns out [..., Hq, Dv]."""
+    nothing).  Returns out [..., Hq, Dv], which must not overlap q, k or v.  States are held
+    to 2^-18 of their terms; of what makes up the outputs, the decayed scores and the state are
+    rounded once to 16 bits on the way (include/catfuse_b200.h has the details)."""
     packed = cu_seqlens is not None
     dev, fmt, Hq, Hk, Dk, Dv, out = _decay_args(q, k, v, log_decay, out, 3 if packed else 4)
     if packed:
@@ -823,7 +825,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     the rotation of their first 2 * len(inv_freq) channels, in one pass ->
     (q_out, k_out); q_out may be q and k_out k.
 
-    positions: int32 or int64, one per token ([...]) or, for several axes (time,
+    positions: contiguous int32 or int64, one per token ([...]) or, for several axes (time,
     height, width), [axes, ...]; sections[a] = number of rotated pairs that
     follow axis a, in whole blocks (``axis_order="blocks"``) or one pair of each
     axis in turn (``"cyclic"``).  Pair p is channels (p, p + rot/2)

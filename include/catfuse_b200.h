@@ -388,14 +388,15 @@ CF_API int cf_pack_conv_weight_planes(const float* w, void* wq, int64_t Cout, in
  * membrane.  With l = exp(log_decay[h]), per head h:
  *     S_t = l * S_{t-1} + k_t^T v_t          S [Dk][Dv] fp32
  *     o_t = scale * q_t S_t
- * log_decay [Hk] fp32 is at most 0 for a leak (-inf: nothing is kept).  The Hq
+ * log_decay [Hk] fp32 is at most 0 for a leak (-inf: nothing is kept, whatever enters).  The Hq
  * query heads come in Hk groups; query head h reads the state of head
  * h / (Hq / Hk).  q, k, v and out are fp16 or bf16 (`fmt`), states fp32
  * [rows][Hk][Dk][Dv].  Tensors are given by the element strides of a token
  * (`_st`) and of a head (`_sh`), channels adjacent, so q, k and v may be slices
  * of one fused projection.  No counterpart in the reference, whose attention
  * (models/spikformer_github.py:147-153) sees all tokens of an image at once.
- * Dk and Dv: multiples of 8, at most 128. */
+ * Dk and Dv: multiples of 8, at most 128.  out must not overlap q, k or v, nor its own
+ * rows each other. */
 
 /* Whole prompts.  N tokens in S sequences: sequence s is tokens
  * [s*L, (s+1)*L) (N = S*L) when cu_seqlens is NULL, else
@@ -410,7 +411,12 @@ CF_API int cf_pack_conv_weight_planes(const float* w, void* wq, int64_t Cout, in
  * reuse once the call's kernels have run.  A non-finite value reaches outputs of
  * its own sequence only, from its own token on (as infinity or NaN).  Rows of q, k and
  * v on 16-byte boundaries (address and strides) run on the tensor cores; other
- * rows take a plain recurrence. */
+ * rows take a plain recurrence.
+ * On the tensor cores states are held to 2^-18 of the sum of their terms' magnitudes.  The
+ * products behind the outputs take the decayed scores and the state rounded once to 16
+ * bits, which makes the outputs' error about 1.4 times that of their own rounding.  In fp16
+ * these factors, and the decayed v behind the state, span 2^39 from the largest of their row (a
+ * token's scores, a state column's v in a chunk of 64 tokens); below that they are lost. */
 CF_API int64_t cf_decay_attention_workspace(int64_t S, int64_t N, int64_t Hq, int64_t Hk, int64_t Dk,
                                             int64_t Dv, int packed);
 CF_API int cf_decay_attention(const void* q, const void* k, const void* v, void* out, int fmt,
@@ -433,8 +439,8 @@ CF_API int cf_decay_attention_step(const void* q, const void* k, const void* v, 
                                    int64_t o_st, int64_t o_sh, float scale, void* stream);
 
 /* Per-head RMS norm of queries and keys and their position rotation, in one
- * pass.  q [N][Hq][D], k [N][Hk][D] and their outputs (which may be q and k) by
- * strides, fp16 or bf16.  norm != 0: x / sqrt(mean(x^2) + eps) * weight, with
+ * pass.  q [N][Hq][D], k [N][Hk][D] and their outputs (which may be q and k; rows of one
+ * output must not overlap) by strides, fp16 or bf16.  norm != 0: x / sqrt(mean(x^2) + eps) * weight, with
  * q_weight / k_weight [D] fp32 (NULL = 1).  The first `rot` channels are rotated
  * in pairs (CF_PAIR_*) by pos * inv_freq[p] (inv_freq [rot/2] fp32), where pos is
  * the token's position on the pair's axis: positions holds `axes` (1 to 4)
